@@ -638,6 +638,44 @@ int nrh_pack_gather(const float* flat, const int* index, const float* factor, lo
 int nrh_sdf32_tables(const float* const* sdf_bias, const int* rows, const float* feat_b, const float* head_b, const float* head_w,
                      float* tables, void* stream);
 
+/* ---- layer operators: networks and per-view tables of any shape (nrhints_amd/ops.py, nrhints_amd/layers.py) ---------------------
+ * The entries above run the networks whose shape is compiled in; these are the same steps - a layer's product, its gradients, a
+ * per-view row for every ray - for any shape, in float32 (dtype 0), float16 (1) or bfloat16 (2).  Tensors are row-major with a row
+ * stride in ELEMENTS (columns contiguous), so a column block of a wider buffer needs no copy; pointers need only be aligned to
+ * their element (16-byte aligned rows are faster).  Sums, bias, activation and residual are float32; each output is rounded once.
+ *
+ * nrh_linear_forward   y [m,n] = act(x [m,k] w [n,k]^T + bias [n]) + residual [m,n]; bias, residual may be null.  activation: 0 none,
+ *   1 ReLU, 2 softplus log(1 + exp(beta z)) / beta, 3 sigmoid, 4 SiLU z sigmoid(z), 5 GELU (erf form).  dact [m,n] (contiguous, may be
+ *   null): act'(z), what the backward entries need.  float32 products are six bfloat16 MFMAs over three-way split operands (float32
+ *   accuracy at any magnitude; tiles with infinities or NaN are computed with float32 MFMAs).
+ * nrh_linear_backward_data     xbar [m,k] = (ybar dact) w
+ * nrh_linear_backward_weight   wbar [n,k] = (ybar dact)^T x, bias_bar [n] = column sums of ybar dact (may be null); m = 0 gives zeros.
+ *   dact: null exactly for activation 0.  For ReLU it is used as a mask: anything positive exactly where z is (y itself, if there was
+ *   no residual).  For 16-bit types ybar dact is rounded to the type before the product (exact for none and ReLU).
+ *   Sums over rows are split in a way that depends on the sizes alone and joined in order: the same bits on every run.
+ * workspace: nrh_linear_workspace_bytes(op = 0 forward, 1 backward_data, 2 backward_weight; ...) bytes, 16-byte aligned; -1: bad
+ *   arguments; 0: none needed.  A workspace belongs to one call at a time.
+ * nrh_embedding_forward    rows [n,d] = scale * table [v,d][index]; index int32 or int64 (index_bits).  An index outside [0, v) stands
+ *   for a slot without a row: zeros.
+ * nrh_embedding_backward   table_bar [v,d] = scale * sum of the rows_bar [n,d] of the tokens that name each row, every row written (zeros
+ *   where no token names it); tokens are sorted by index and summed in a fixed order, without atomics: the same bits on every run. */
+long long nrh_linear_workspace_bytes(int op, int dtype, long long m, long long n, long long k);
+int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* residual,
+                       long long ldr, int activation, float beta, long long m, long long n, long long k, void* y, long long ldy,
+                       void* dact, void* workspace, long long workspace_bytes, void* stream);
+int nrh_linear_backward_data(int dtype, const void* ybar, long long ldyb, const void* dact, long long ldd, int activation, const void* w,
+                             long long ldw, long long m, long long n, long long k, void* xbar, long long ldxb, void* workspace,
+                             long long workspace_bytes, void* stream);
+int nrh_linear_backward_weight(int dtype, const void* ybar, long long ldyb, const void* dact, long long ldd, int activation, const void* x,
+                               long long ldx, long long m, long long n, long long k, void* wbar, long long ldwb, void* bias_bar,
+                               void* workspace, long long workspace_bytes, void* stream);
+int nrh_embedding_forward(int dtype, const void* table, long long ldt, long long v, long long d, const void* index, int index_bits,
+                          long long n, float scale, void* rows, long long ldr, void* stream);
+long long nrh_embedding_backward_workspace_bytes(long long n, long long v, long long d);
+int nrh_embedding_backward(int dtype, const void* rows_bar, long long ldr, const void* index, int index_bits, long long n, long long v,
+                           long long d, float scale, void* table_bar, long long ldt, void* workspace, long long workspace_bytes,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -30,7 +30,9 @@ EXPORTED = ("nrh_version", "nrh_build_info", "nrh_source_hash", "nrh_last_error_
             "nrh_dw_workspace_floats", "nrh_dw_gemm", "nrh_embedding_rows", "nrh_composite_loss", "nrh_loss_finish",
             "nrh_alpha_train_backward_fused", "nrh_variance_grad", "nrh_pack_gather", "nrh_sdf32_tables", "nrh_adam_step", "nrh_fuse_feature_head",
             "nrh_train_arrays_tiled", "nrh_sdf_eval_wide_f16", "nrh_train_half_supported", "nrh_sdf_train_forward_half",
-            "nrh_sdf_train_backward_half", "nrh_color_train_forward_half", "nrh_color_train_backward_half", "nrh_step_scalars", "nrh_sampler_fusion")
+            "nrh_sdf_train_backward_half", "nrh_color_train_forward_half", "nrh_color_train_backward_half", "nrh_step_scalars", "nrh_sampler_fusion",
+            "nrh_linear_workspace_bytes", "nrh_linear_forward", "nrh_linear_backward_data", "nrh_linear_backward_weight",
+            "nrh_embedding_forward", "nrh_embedding_backward_workspace_bytes", "nrh_embedding_backward")
 
 
 class NrhNet(Structure):
@@ -231,6 +233,16 @@ def load():
     lib.nrh_sampler_fusion.argtypes = [c_int]
     lib.nrh_sampler_fusion.restype = c_int
     lib.nrh_kernel_timing_read.argtypes = [POINTER(ctypes.c_double), POINTER(c_longlong)]
+    L = c_longlong
+    lib.nrh_linear_workspace_bytes.argtypes = [c_int, c_int, L, L, L]
+    lib.nrh_linear_workspace_bytes.restype = L
+    lib.nrh_linear_forward.argtypes = [c_int, P, L, P, L, P, P, L, c_int, c_float, L, L, L, P, L, P, P, L, P]
+    lib.nrh_linear_backward_data.argtypes = [c_int, P, L, P, L, c_int, P, L, L, L, L, P, L, P, L, P]
+    lib.nrh_linear_backward_weight.argtypes = [c_int, P, L, P, L, c_int, P, L, L, L, L, P, L, P, P, L, P]
+    lib.nrh_embedding_forward.argtypes = [c_int, P, L, L, L, P, c_int, L, c_float, P, L, P]
+    lib.nrh_embedding_backward_workspace_bytes.argtypes = [L, L, L]
+    lib.nrh_embedding_backward_workspace_bytes.restype = L
+    lib.nrh_embedding_backward.argtypes = [c_int, P, L, P, c_int, L, L, L, c_float, P, L, P, L, P]
     for name in EXPORTED:
         getattr(lib, name)  # AttributeError if the build is stale
     _lib = lib

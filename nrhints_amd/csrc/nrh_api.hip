@@ -23,6 +23,7 @@
 #include "../../include/nrhints_hip.h"
 #include "nrh_wide.h"
 #include "nrh_small.h"
+#include "nrh_layers.h"
 
 namespace {
 
@@ -1840,6 +1841,145 @@ int nrh_render_forward_train(const NrhNet* net, const float* origins, const floa
                              t_rand_shadow, zero_hints, lin64, lin16, nullptr, depth, weights, inside_sphere, analytic_normals,
                              normalized_normals, visibilities, specular_cue, mid_z, dists, nullptr, nullptr, saves, workspace,
                              workspace_floats, stream);
+}
+
+// ---- layer operators (nrh_linear.hip, nrh_embedding.hip) --------------------------------------------------------------------
+static int layer_result(int rc, const char* who) {
+  if (rc == -3) return fail(NRH_E_WORKSPACE, "%s: workspace too small", who);
+  if (rc) return fail(NRH_E_LAUNCH, "%s: launch failed", who);
+  return NRH_OK;
+}
+
+static bool off_element(const void* p, int dtype) { return ((uintptr_t)p % (dtype == 0 ? 4 : 2)) != 0; }
+
+static int linear_sizes(const char* who, int dtype, int act, long long m, long long n, long long k) {
+  if (dtype < 0 || dtype > 2) return fail(NRH_E_INVALID, "%s: dtype must be 0 (float32), 1 (float16) or 2 (bfloat16)", who);
+  if (act < 0 || act > 5) return fail(NRH_E_INVALID, "%s: unknown activation", who);
+  if (m < 0 || n < 1 || k < 1) return fail(NRH_E_INVALID, "%s: sizes must be m >= 0, n >= 1, k >= 1", who);
+  if (m > (1LL << 30) || n > (1LL << 20) || k > (1LL << 20) || ((m + 63) / 64) * ((n + 63) / 64) > (1LL << 23) ||
+      ((m + 63) / 64) * ((k + 63) / 64) > (1LL << 23) || ((n + 63) / 64) * ((k + 63) / 64) > (1LL << 23))
+    return fail(NRH_E_INVALID, "%s: too large (at most 2^30 rows, 2^20 columns and 2^23 tiles of 64 x 64)", who);
+  return NRH_OK;
+}
+
+long long nrh_linear_workspace_bytes(int op, int dtype, long long m, long long n, long long k) {
+  if (op < 0 || op > 2 || dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1) return -1;
+  return nrhlin::workspace_bytes(op, dtype, m, n, k);
+}
+
+int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* residual,
+                       long long ldr, int activation, float beta, long long m, long long n, long long k, void* y, long long ldy,
+                       void* dact, void* workspace, long long workspace_bytes, void* stream) {
+  const char* who = "nrh_linear_forward";
+  const int rc = linear_sizes(who, dtype, activation, m, n, k);
+  if (rc) return rc;
+  if (m == 0) return NRH_OK;
+  if (!x || !w || !y) return fail(NRH_E_INVALID, "%s: null pointer", who);
+  if (ldx < k || ldw < k || ldy < n || (residual && ldr < n)) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
+  if (activation == nrhlin::SOFTPLUS && !(beta > 0.0f && beta < 1e30f)) return fail(NRH_E_INVALID, "%s: softplus needs a positive beta", who);
+  if (off_element(x, dtype) || off_element(w, dtype) || off_element(y, dtype) || off_element(bias, dtype) || off_element(residual, dtype) ||
+      off_element(dact, dtype))
+    return fail(NRH_E_INVALID, "%s: a pointer is not aligned to its element", who);
+  nrhlin::Call c = {};
+  c.op = nrhlin::FORWARD;
+  c.dtype = dtype;
+  c.act = activation;
+  c.beta = beta;
+  c.m = m; c.n = n; c.k = k;
+  c.x = x; c.ldx = ldx;
+  c.w = w; c.ldw = ldw;
+  c.bias = bias;
+  c.res = residual; c.ldr = ldr;
+  c.out = y; c.ldo = ldy;
+  c.dact_out = dact;
+  c.ws = workspace; c.ws_bytes = workspace_bytes;
+  return layer_result(nrhlin::launch(c, (hipStream_t)stream), who);
+}
+
+static int linear_backward(int op, const char* who, int dtype, const void* ybar, long long ldyb, const void* dact, long long ldd,
+                           int activation, const void* other, long long ldother, long long m, long long n, long long k, void* out,
+                           long long ldo, void* bias_bar, void* workspace, long long workspace_bytes, void* stream) {
+  const int rc = linear_sizes(who, dtype, activation, m, n, k);
+  if (rc) return rc;
+  if (m == 0 && op == nrhlin::BACK_DATA) return NRH_OK;
+  if (!out || (m > 0 && (!ybar || !other))) return fail(NRH_E_INVALID, "%s: null pointer", who);
+  if (m > 0 && (activation == nrhlin::NONE) != (dact == nullptr))
+    return fail(NRH_E_INVALID, "%s: the saved derivative is needed exactly when there is an activation", who);
+  if (ldyb < n || (dact && ldd < n) || ldother < k || ldo < k) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
+  if (off_element(ybar, dtype) || off_element(dact, dtype) || off_element(other, dtype) || off_element(out, dtype) || off_element(bias_bar, dtype))
+    return fail(NRH_E_INVALID, "%s: a pointer is not aligned to its element", who);
+  nrhlin::Call c = {};
+  c.op = op;
+  c.dtype = dtype;
+  c.act = activation;
+  c.m = m; c.n = n; c.k = k;
+  if (op == nrhlin::BACK_DATA) { c.w = other; c.ldw = ldother; }
+  else { c.x = other; c.ldx = ldother; }
+  c.ybar = ybar; c.ldyb = ldyb;
+  c.dact = dact; c.ldd = ldd;
+  c.out = out; c.ldo = ldo;
+  c.bias_bar = bias_bar;
+  c.ws = workspace; c.ws_bytes = workspace_bytes;
+  return layer_result(nrhlin::launch(c, (hipStream_t)stream), who);
+}
+
+int nrh_linear_backward_data(int dtype, const void* ybar, long long ldyb, const void* dact, long long ldd, int activation, const void* w,
+                             long long ldw, long long m, long long n, long long k, void* xbar, long long ldxb, void* workspace,
+                             long long workspace_bytes, void* stream) {
+  return linear_backward(nrhlin::BACK_DATA, "nrh_linear_backward_data", dtype, ybar, ldyb, dact, ldd, activation, w, ldw, m, n, k, xbar, ldxb,
+                         nullptr, workspace, workspace_bytes, stream);
+}
+
+int nrh_linear_backward_weight(int dtype, const void* ybar, long long ldyb, const void* dact, long long ldd, int activation, const void* x,
+                               long long ldx, long long m, long long n, long long k, void* wbar, long long ldwb, void* bias_bar,
+                               void* workspace, long long workspace_bytes, void* stream) {
+  return linear_backward(nrhlin::BACK_WEIGHT, "nrh_linear_backward_weight", dtype, ybar, ldyb, dact, ldd, activation, x, ldx, m, n, k, wbar,
+                         ldwb, bias_bar, workspace, workspace_bytes, stream);
+}
+
+static int embedding_call(const char* who, int dtype, int index_bits, const void* index, long long n, long long v, long long d, float scale,
+                          const void* src, long long lds, void* dst, long long ldd, nrhemb::Call& c) {
+  if (dtype < 0 || dtype > 2) return fail(NRH_E_INVALID, "%s: dtype must be 0 (float32), 1 (float16) or 2 (bfloat16)", who);
+  if (index_bits != 32 && index_bits != 64) return fail(NRH_E_INVALID, "%s: the index must be int32 or int64", who);
+  if (n < 0 || v < 1 || d < 1) return fail(NRH_E_INVALID, "%s: sizes must be n >= 0, v >= 1, d >= 1", who);
+  if (n > (1LL << 30) || v > (1LL << 31) - 2 || d > (1LL << 20)) return fail(NRH_E_INVALID, "%s: too large (at most 2^30 tokens, 2^31 - 2 rows, 2^20 columns)", who);
+  if (lds < d || ldd < d) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
+  if (off_element(src, dtype) || off_element(dst, dtype) || (index && (uintptr_t)index % (index_bits / 8) != 0))
+    return fail(NRH_E_INVALID, "%s: a pointer is not aligned to its element", who);
+  c = {};
+  c.dtype = dtype;
+  c.index64 = index_bits == 64;
+  c.index = index;
+  c.n = n; c.v = v; c.d = d;
+  c.scale = scale;
+  c.src = src; c.lds = lds;
+  c.dst = dst; c.ldd = ldd;
+  return NRH_OK;
+}
+
+int nrh_embedding_forward(int dtype, const void* table, long long ldt, long long v, long long d, const void* index, int index_bits, long long n,
+                          float scale, void* rows, long long ldr, void* stream) {
+  const char* who = "nrh_embedding_forward";
+  nrhemb::Call c;
+  const int rc = embedding_call(who, dtype, index_bits, index, n, v, d, scale, table, ldt, rows, ldr, c);
+  if (rc || n == 0) return rc;
+  if (!table || !index || !rows) return fail(NRH_E_INVALID, "%s: null pointer", who);
+  return layer_result(nrhemb::forward(c, (hipStream_t)stream), who);
+}
+
+long long nrh_embedding_backward_workspace_bytes(long long n, long long v, long long d) {
+  return n < 0 || v < 1 || d < 1 ? -1 : nrhemb::backward_workspace_bytes(n, v, d);
+}
+
+int nrh_embedding_backward(int dtype, const void* rows_bar, long long ldr, const void* index, int index_bits, long long n, long long v,
+                           long long d, float scale, void* table_bar, long long ldt, void* workspace, long long workspace_bytes, void* stream) {
+  const char* who = "nrh_embedding_backward";
+  nrhemb::Call c;
+  const int rc = embedding_call(who, dtype, index_bits, index, n, v, d, scale, rows_bar, ldr, table_bar, ldt, c);
+  if (rc) return rc;
+  if (!table_bar || (n > 0 && (!rows_bar || !index))) return fail(NRH_E_INVALID, "%s: null pointer", who);
+  c.ws = workspace; c.ws_bytes = workspace_bytes;
+  return layer_result(nrhemb::backward(c, (hipStream_t)stream), who);
 }
 
 }  // extern "C"

@@ -1,0 +1,433 @@
+// Table lookup with scaling,  rows[i] = s T[idx[i]],  and its gradient  Tbar[v] = s sum_{idx[i] = v} rowsbar[i].
+//
+// The gradient sorts the tokens by index - stable, so a row's tokens stay in their order - and sums runs of equal index: no atomics on
+// floating point numbers, the same bits on every run, float32 sums, one rounding.
+//   sort      up to 2 048 tokens: bitonic in LDS, one launch; more: least significant digit first, 8 bits per pass (histogram of a
+//             tile of 2 048 tokens, scan per digit, ranked scatter), as many passes as the table's height has digits.
+//   zero      rows that no token names, found by bisection in the sorted keys (the others are written once, by the sums).
+//   sum       a group of lanes - one lane per 16 bytes of a row - walks 32 sorted tokens.  A run that begins and ends inside is
+//             written to the table; the first and the last run of a group may go on in its neighbours and are handed, as float32
+//             rows with their keys, to the next level, which does the same with 1/16 of the entries until one group is left.  A row
+//             named by every token and a table named once per row cost the same.
+// Both directions are bound by HBM: the tokens' rows are read once, the table's gradient is written once.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "nrh_layers.h"
+
+namespace nrhemb {
+
+typedef long long ll;
+typedef unsigned long long ull;
+constexpr unsigned NONE = 0xffffffffu;
+constexpr int TILE = 2048, SMALL = 2048, RUN = 32;
+
+template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
+template <typename T> struct Vec<T, 1> { typedef T type; };
+template <typename T, int V> __device__ __forceinline__ float at(const typename Vec<T, V>::type& x, int e) {
+  if constexpr (V == 1) return (float)x;
+  else return (float)x[e];
+}
+template <typename T, int V> __device__ __forceinline__ void put(typename Vec<T, V>::type& x, int e, float f) {
+  if constexpr (V == 1) x = (T)f;
+  else x[e] = (T)f;
+}
+
+__device__ __forceinline__ ll load_index(const void* index, int index64, ll i) {
+  return index64 ? ((const ll*)index)[i] : (ll)((const int*)index)[i];
+}
+
+// one lane per V columns of a row
+template <typename T, int V>
+__global__ __launch_bounds__(256) void lookup_kernel(const void* index, int index64, ll n, ll v, int cols, float scale, const T* __restrict__ table,
+                                                     ll ldt, T* __restrict__ rows, ll ldr) {
+  typedef typename Vec<T, V>::type VT;
+  for (ll e = (ll)blockIdx.x * 256 + threadIdx.x; e < n * cols; e += (ll)gridDim.x * 256) {
+    const ll i = e / cols, c = (e % cols) * V;
+    const ll k = load_index(index, index64, i);
+    VT y = {};
+    if (k >= 0 && k < v) {
+      const VT x = *(const VT*)(table + k * ldt + c);
+#pragma unroll
+      for (int q = 0; q < V; ++q) put<T, V>(y, q, scale * at<T, V>(x, q));
+    }
+    *(VT*)(rows + i * ldr + c) = y;
+  }
+}
+
+// ---- sort --------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ unsigned key_of(const void* index, int index64, ll i, ll v) {
+  const ll k = load_index(index, index64, i);
+  return (unsigned)(k >= 0 && k < v ? k : v);
+}
+
+__global__ __launch_bounds__(1024) void sort_small_kernel(const void* index, int index64, int n, ll v, unsigned* keys, unsigned* perm) {
+  __shared__ ull a[SMALL];
+  const int tid = threadIdx.x;
+  int m = 2;
+  while (m < n) m *= 2;
+  for (int i = tid; i < m; i += 1024) a[i] = i < n ? ((ull)key_of(index, index64, i, v) << 32) | (unsigned)i : ~0ull;
+  for (int k = 2; k <= m; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      for (int t = tid; t < m / 2; t += 1024) {
+        const int lo = 2 * t - (t & (j - 1)), hi = lo + j;
+        const ull x = a[lo], y = a[hi];
+        if ((x > y) == ((lo & k) == 0)) {
+          a[lo] = y;
+          a[hi] = x;
+        }
+      }
+    }
+  __syncthreads();
+  for (int i = tid; i < n; i += 1024) {
+    keys[i] = (unsigned)(a[i] >> 32);
+    perm[i] = (unsigned)a[i];
+  }
+}
+
+struct Pass {
+  const void* index;      // first pass: keys come from the caller's index, positions count up
+  int index64, first, shift;
+  ll n, v;
+  const unsigned *keys_in, *perm_in;
+  unsigned *keys_out, *perm_out;
+  unsigned *hist, *total;  // [256][tiles], [256]
+  ll tiles;
+};
+
+__device__ __forceinline__ unsigned pass_key(const Pass& p, ll i) { return p.first ? key_of(p.index, p.index64, i, p.v) : p.keys_in[i]; }
+
+__global__ __launch_bounds__(256) void hist_kernel(const Pass p) {
+  __shared__ unsigned h[256];
+  h[threadIdx.x] = 0;
+  __syncthreads();
+  const ll base = (ll)blockIdx.x * TILE;
+  for (int r = 0; r < TILE / 256; ++r) {
+    const ll i = base + r * 256 + threadIdx.x;
+    if (i < p.n) atomicAdd(&h[(pass_key(p, i) >> p.shift) & 255], 1u);      // counts: the order does not matter
+  }
+  __syncthreads();
+  p.hist[(ll)threadIdx.x * p.tiles + blockIdx.x] = h[threadIdx.x];
+}
+
+// exclusive scan over 256 values, one per thread; buf [256]
+__device__ __forceinline__ unsigned scan256(unsigned x, unsigned* buf, unsigned& total) {
+  const int t = threadIdx.x;
+  __syncthreads();
+  buf[t] = x;
+  __syncthreads();
+  for (int d = 1; d < 256; d *= 2) {
+    const unsigned y = t >= d ? buf[t - d] : 0;
+    __syncthreads();
+    buf[t] += y;
+    __syncthreads();
+  }
+  total = buf[255];
+  return buf[t] - x;
+}
+
+__global__ __launch_bounds__(256) void scan_kernel(const Pass p) {
+  __shared__ unsigned buf[256];
+  unsigned* h = p.hist + (ll)blockIdx.x * p.tiles;
+  unsigned carry = 0;
+  for (ll b = 0; b < p.tiles; b += 256) {
+    const ll i = b + threadIdx.x;
+    unsigned total;
+    const unsigned ex = scan256(i < p.tiles ? h[i] : 0, buf, total);
+    if (i < p.tiles) h[i] = carry + ex;
+    carry += total;
+  }
+  if (threadIdx.x == 0) p.total[blockIdx.x] = carry;
+}
+
+__global__ __launch_bounds__(256) void scatter_kernel(const Pass p) {
+  constexpr int ROUNDS = TILE / 256;
+  __shared__ unsigned cnt[4][256];
+  __shared__ unsigned buf[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+  unsigned all;
+  const unsigned digit_base = scan256(p.total[tid], buf, all) + p.hist[(ll)tid * p.tiles + blockIdx.x];
+  __syncthreads();
+  volatile unsigned* mine = cnt[wave];
+  const ll base = (ll)blockIdx.x * TILE + wave * (TILE / 4);
+  unsigned key[ROUNDS], rank[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const ll i = base + r * 64 + lane;
+    const bool live = i < p.n;
+    key[r] = live ? pass_key(p, i) : 0;
+    const unsigned d = (key[r] >> p.shift) & 255;
+    ull peers = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const ull on = __ballot((d >> b) & 1);
+      peers &= (d >> b) & 1 ? on : ~on;
+    }
+    const unsigned before = (unsigned)__popcll(peers & ((1ull << lane) - 1));
+    if (live) {
+      const unsigned c = mine[d];
+      rank[r] = c + before;
+      if (before == 0) mine[d] = c + (unsigned)__popcll(peers);
+    }
+  }
+  __syncthreads();
+  unsigned c = digit_base;
+  for (int w = 0; w < 4; ++w) {
+    const unsigned x = cnt[w][tid];
+    cnt[w][tid] = c;
+    c += x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const ll i = base + r * 64 + lane;
+    if (i < p.n) {
+      const unsigned to = cnt[wave][(key[r] >> p.shift) & 255] + rank[r];
+      p.keys_out[to] = key[r];
+      p.perm_out[to] = p.first ? (unsigned)i : p.perm_in[i];
+    }
+  }
+}
+
+// ---- sums --------------------------------------------------------------------------------------------------------------------
+// one wave per table row (and 64 V columns at a time): zeros where no sorted key equals the row
+template <typename T, int V>
+__global__ __launch_bounds__(256) void zero_kernel(const unsigned* __restrict__ keys, ll n, ll v, int cols, T* __restrict__ out, ll ldo) {
+  typedef typename Vec<T, V>::type VT;
+  for (ll row = (ll)blockIdx.x * 4 + (threadIdx.x >> 6); row < v; row += (ll)gridDim.x * 4) {
+    ll lo = 0, hi = n;
+    while (lo < hi) {
+      const ll mid = (lo + hi) / 2;
+      if (keys[mid] < (unsigned)row) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo < n && keys[lo] == (unsigned)row) continue;
+    const VT z = {};
+    for (int c = threadIdx.x & 63; c < cols; c += 64) *(VT*)(out + row * ldo + (ll)c * V) = z;
+  }
+}
+
+struct Level {
+  const unsigned *keys, *perm;   // perm: first level only
+  const void* rows;              // first level: T [.., ldr], else float [n][d]
+  ll ldr, n, v;
+  int d, cols, width;            // cols: vectors per row; width: lanes per group
+  float scale;
+  void* out;
+  ll ldo;
+  unsigned* next_keys;           // null: the last level
+  float* next_rows;
+};
+
+template <typename T, int V, bool FIRST>
+__global__ __launch_bounds__(256) void sum_kernel(const Level a) {
+  typedef typename Vec<T, V>::type VT;
+  typedef typename Vec<float, V>::type FT;
+  constexpr int BATCH = 8;
+  const ll g = (ll)blockIdx.x * (256 / a.width) + threadIdx.x / a.width;
+  const int c = blockIdx.y * a.width + threadIdx.x % a.width;
+  const ll beg = g * RUN, end = beg + RUN < a.n ? beg + RUN : a.n;
+  if (beg >= a.n || c >= a.cols) return;
+  const ll col = (ll)c * V;
+  unsigned cur = NONE;
+  bool head = true;              // the run in hand is the group's first
+  float acc[V];
+#pragma unroll
+  for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+  auto to_table = [&](unsigned k) {
+    VT y;
+#pragma unroll
+    for (int q = 0; q < V; ++q) put<T, V>(y, q, a.scale * acc[q]);
+    *(VT*)((T*)a.out + (ll)k * a.ldo + col) = y;
+  };
+  auto to_next = [&](ll slot, unsigned k) {
+    if (c == 0) a.next_keys[slot] = k;
+    if (k == NONE) return;
+    FT y;
+#pragma unroll
+    for (int q = 0; q < V; ++q) put<float, V>(y, q, acc[q]);
+    *(FT*)(a.next_rows + slot * a.d + col) = y;
+  };
+  for (ll e = beg; e < end; e += BATCH) {
+    unsigned k[BATCH];
+    float x[BATCH][V];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      k[b] = e + b < end ? a.keys[e + b] : NONE;
+      if (FIRST && k[b] >= (unsigned)a.v) k[b] = NONE;       // tokens that name no row
+    }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b)
+      if (k[b] != NONE) {
+        if constexpr (FIRST) {
+          const VT y = *(const VT*)((const T*)a.rows + (ll)a.perm[e + b] * a.ldr + col);
+#pragma unroll
+          for (int q = 0; q < V; ++q) x[b][q] = at<T, V>(y, q);
+        } else {
+          const FT y = *(const FT*)((const float*)a.rows + (e + b) * a.ldr + col);
+#pragma unroll
+          for (int q = 0; q < V; ++q) x[b][q] = at<float, V>(y, q);
+        }
+      }
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      if (k[b] == NONE) continue;
+      if (k[b] != cur) {
+        if (cur != NONE) {
+          if (head && a.next_keys) to_next(2 * g, cur);
+          else to_table(cur);
+          head = false;
+        }
+        cur = k[b];
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] += x[b][q];
+    }
+  }
+  if (!a.next_keys) {
+    if (cur != NONE) to_table(cur);
+    return;
+  }
+  if (head) {
+    to_next(2 * g, cur);
+    to_next(2 * g + 1, NONE);
+  } else {
+    to_next(2 * g + 1, cur);
+  }
+}
+
+// ---- host --------------------------------------------------------------------------------------------------------------------
+static ll align256(ll x) { return (x + 255) / 256 * 256; }
+static ll groups(ll n) { return (n + RUN - 1) / RUN; }
+
+struct Layout {
+  ll keys[2], perm[2], hist, total, lkeys[2], lrows[2], bytes;
+};
+
+static Layout layout(ll n, ll d) {
+  Layout l;
+  ll at = 0;
+  auto take = [&](ll bytes) {
+    const ll here = at;
+    at += align256(bytes);
+    return here;
+  };
+  for (int b = 0; b < 2; ++b) {
+    l.keys[b] = take(4 * n);
+    l.perm[b] = take(4 * n);
+  }
+  l.hist = take(1024 * ((n + TILE - 1) / TILE));
+  l.total = take(1024);
+  const ll n1 = 2 * groups(n), n2 = 2 * groups(n1);
+  l.lkeys[0] = take(4 * n1);
+  l.lrows[0] = take(4 * n1 * d);
+  l.lkeys[1] = take(4 * n2);
+  l.lrows[1] = take(4 * n2 * d);
+  l.bytes = at;
+  return l;
+}
+
+long long backward_workspace_bytes(long long n, long long v, long long d) {
+  (void)v;
+  return n <= 0 ? 0 : layout(n, d).bytes;
+}
+
+// a grid's threads are counted in 32 bits: larger ranges loop
+static dim3 blocks(ll n) { return dim3((unsigned)(n < (1 << 22) ? n : (1 << 22))); }
+
+static bool vec_ok(const void* p, ll ld, ll d, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0 && (d * es) % 16 == 0; }
+
+template <typename T, int V> static int forward_as(const Call& c, hipStream_t st) {
+  const ll cols = c.d / V;
+  lookup_kernel<T, V><<<blocks((c.n * cols + 255) / 256), 256, 0, st>>>(c.index, c.index64, c.n, c.v, (int)cols, c.scale,
+                                                                                  (const T*)c.src, c.lds, (T*)c.dst, c.ldd);
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+template <typename T, int V> static int backward_as(const Call& c, hipStream_t st) {
+  const int cols = (int)(c.d / V);
+  const Layout l = layout(c.n, c.d);
+  if (c.n > 0 && (!c.ws || c.ws_bytes < l.bytes)) return -3;
+  char* ws = (char*)c.ws;
+  unsigned *keys[2], *perm[2];
+  for (int b = 0; b < 2; ++b) {
+    keys[b] = (unsigned*)(ws + l.keys[b]);
+    perm[b] = (unsigned*)(ws + l.perm[b]);
+  }
+  int cur = 0;
+  if (c.n > 0 && c.n <= SMALL) {
+    sort_small_kernel<<<1, 1024, 0, st>>>(c.index, c.index64, (int)c.n, c.v, keys[0], perm[0]);
+  } else if (c.n > 0) {
+    Pass p;
+    p.index = c.index;
+    p.index64 = c.index64;
+    p.n = c.n;
+    p.v = c.v;
+    p.hist = (unsigned*)(ws + l.hist);
+    p.total = (unsigned*)(ws + l.total);
+    p.tiles = (c.n + TILE - 1) / TILE;
+    int bits = 1;
+    while (bits < 32 && (c.v >> bits) != 0) ++bits;           // keys 0 .. v
+    for (p.shift = 0; p.shift < bits; p.shift += 8) {
+      p.first = p.shift == 0;
+      p.keys_in = keys[1 - cur];
+      p.perm_in = perm[1 - cur];
+      p.keys_out = keys[cur];
+      p.perm_out = perm[cur];
+      hist_kernel<<<dim3((unsigned)p.tiles), 256, 0, st>>>(p);
+      scan_kernel<<<256, 256, 0, st>>>(p);
+      scatter_kernel<<<dim3((unsigned)p.tiles), 256, 0, st>>>(p);
+      cur = 1 - cur;
+    }
+    cur = 1 - cur;
+  }
+  zero_kernel<T, V><<<blocks((c.v + 3) / 4), 256, 0, st>>>(keys[cur], c.n, c.v, cols, (T*)c.dst, c.ldd);
+  Level a;
+  a.v = c.v;
+  a.d = (int)c.d;
+  a.cols = cols;
+  a.width = 1;
+  while (a.width < cols && a.width < 64) a.width *= 2;
+  a.scale = c.scale;
+  a.out = c.dst;
+  a.ldo = c.ldd;
+  ll n = c.n;
+  for (int level = 0; n > 0; ++level) {
+    const ll g = groups(n);
+    const bool last = g == 1;
+    a.n = n;
+    a.keys = level == 0 ? keys[cur] : (const unsigned*)(ws + l.lkeys[(level - 1) & 1]);
+    a.perm = perm[cur];
+    a.rows = level == 0 ? c.src : (const void*)(ws + l.lrows[(level - 1) & 1]);
+    a.ldr = level == 0 ? c.lds : c.d;
+    a.next_keys = last ? nullptr : (unsigned*)(ws + l.lkeys[level & 1]);
+    a.next_rows = (float*)(ws + l.lrows[level & 1]);
+    const int per = 256 / a.width;
+    const dim3 grid((unsigned)((g + per - 1) / per), (unsigned)((cols + a.width - 1) / a.width));
+    if (level == 0) sum_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
+    else sum_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
+    n = last ? 0 : 2 * g;
+  }
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
+int forward(const Call& c, hipStream_t st) {
+  const int es = c.dtype == nrhlin::F32 ? 4 : 2;
+  const bool vec = vec_ok(c.src, c.lds, c.d, es) && vec_ok(c.dst, c.ldd, c.d, es);
+  if (c.dtype == nrhlin::F32) return vec ? forward_as<float, 4>(c, st) : forward_as<float, 1>(c, st);
+  if (c.dtype == nrhlin::F16) return vec ? forward_as<_Float16, 8>(c, st) : forward_as<_Float16, 1>(c, st);
+  return vec ? forward_as<__bf16, 8>(c, st) : forward_as<__bf16, 1>(c, st);
+}
+
+int backward(const Call& c, hipStream_t st) {
+  const int es = c.dtype == nrhlin::F32 ? 4 : 2;
+  const bool vec = vec_ok(c.src, c.lds, c.d, es) && vec_ok(c.dst, c.ldd, c.d, es);
+  if (c.dtype == nrhlin::F32) return vec ? backward_as<float, 4>(c, st) : backward_as<float, 1>(c, st);
+  if (c.dtype == nrhlin::F16) return vec ? backward_as<_Float16, 8>(c, st) : backward_as<_Float16, 1>(c, st);
+  return vec ? backward_as<__bf16, 8>(c, st) : backward_as<__bf16, 1>(c, st);
+}
+
+}  // namespace nrhemb

@@ -3,6 +3,10 @@
 ``NeuSHintRenderer.forward`` does not use these (it makes one fused C call per chunk); they exist so that each
 kernel can be parity-tested in isolation and so that callers such as mesh extraction can query the SDF alone.
 All tensors are float32, contiguous, on the GPU.  No fallback: errors raise.
+
+The last section holds the layer operators, which take networks and tables of ANY shape in float32, float16 or bfloat16: ``linear`` (a
+layer's product with bias, activation and residual) and ``embedding`` (rows of a table, scaled) with their gradients.  They work on
+plain tensors and record no autograd graph; ``nrhints_amd.layers`` wraps them for autograd.
 """
 from __future__ import annotations
 
@@ -288,3 +292,173 @@ def color_composite(color, weights, wsum, background=None, inside=None, grad=Non
                                  _lib.stream_handle())
     _lib.check(rc, "nrh_color_composite")
     return rgb, nm, nnm
+
+
+# ---- layer operators -------------------------------------------------------------------------------------------------------------
+#: activation names of ``linear`` in the order of the C entry's codes
+ACTIVATIONS = ("none", "relu", "softplus", "sigmoid", "silu", "gelu")
+_ACT = {name: code for code, name in enumerate(ACTIVATIONS)}
+_DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` as a [rows, cols] matrix of contiguous rows on ``like``'s device and of its type: a view where the strides allow it (a
+    column block of a wider buffer), else a copy."""
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{what}: expected a {like.dtype} tensor on {like.device}, got {getattr(t, 'dtype', type(t))} on {getattr(t, 'device', None)}")
+    if t.dim() != 2:
+        t = t.reshape(rows, cols)
+    if (t.stride(1) != 1 and cols > 1) or (t.stride(0) < cols and rows > 1):
+        t = t.contiguous()
+    return t
+
+
+def _ld(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _layer_input(x: torch.Tensor, what: str) -> int:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{what}: expected a tensor on the GPU (there is no CPU path)")
+    if x.dtype not in _DTYPE:
+        raise ValueError(f"{what}: float32, float16 or bfloat16, got {x.dtype}")
+    return _DTYPE[x.dtype]
+
+
+def _linear_shapes(x, weight, activation):
+    code = _ACT.get(activation)
+    if code is None:
+        raise ValueError(f"unknown activation {activation!r}: one of {', '.join(ACTIVATIONS)}")
+    dtype = _layer_input(x, "x")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"linear: x [..., k] and weight [n, k] with n, k >= 1, got {tuple(x.shape)} and {tuple(getattr(weight, 'shape', ()))}")
+    n, k = weight.shape
+    return dtype, code, x.numel() // k, n, k
+
+
+def _workspace(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _vp(t):
+    return None if t is None else t.data_ptr()
+
+
+def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
+    dtype, code, m, n, k = _linear_shapes(x, weight, activation)
+    if code == 2 and not 0.0 < float(beta) < 1e30:
+        raise ValueError("linear: softplus needs a positive beta")
+    x2, w2 = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight")
+    shape = x.shape[:-1] + (n,)
+    if bias is not None and bias.shape != (n,):
+        raise ValueError(f"linear: bias must be [{n}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)} (it is not broadcast)")
+    b1 = None if bias is None else _matrix(bias.reshape(1, n), 1, n, x, "bias")
+    r2 = None if residual is None else _matrix(residual, m, n, x, "residual")
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    keep = want_dact and code != 0 and not (code == 1 and residual is None)
+    dact = torch.empty(shape, dtype=x.dtype, device=x.device) if keep else None
+    lib = _lib.load()
+    with torch.cuda.device(x.device):
+        nbytes = lib.nrh_linear_workspace_bytes(0, dtype, m, n, k)
+        ws = _workspace(nbytes, x.device)
+        _lib.check(lib.nrh_linear_forward(dtype, _vp(x2), _ld(x2), _vp(w2), _ld(w2), _vp(b1), _vp(r2), 0 if r2 is None else _ld(r2), code,
+                                          float(beta), m, n, k, _vp(y), n, _vp(dact), _vp(ws), nbytes, _lib.stream_handle()),
+                   "nrh_linear_forward")
+    if want_dact and code == 1 and residual is None:
+        dact = y           # ReLU: the output is positive exactly where the argument is
+    return y, dact
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+           activation: str = "none", beta: float = 100.0) -> torch.Tensor:
+    """``act(x weight^T + bias) + residual`` in one launch (two where few rows meet a long reduction): x [..., k], weight [n, k],
+    bias [n], residual of the output's shape; activation one of ``ACTIVATIONS``, softplus with ``beta`` (the SDF network's 100,
+    fields/sdf_field.py:104).  One type for all tensors, float32 inside, one rounding.  Row strides are taken as they are; other
+    strides are copied.  -> y [..., n] (contiguous)."""
+    return _linear_forward(x, weight, bias, residual, activation, beta, False)[0]
+
+
+def linear_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                         residual: Optional[torch.Tensor] = None, activation: str = "none",
+                         beta: float = 100.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) in the tensors' type, None for
+    "none", and y itself for "relu" without a residual (do not change y in place before the backward then)."""
+    return _linear_forward(x, weight, bias, residual, activation, beta, True)
+
+
+def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, dact: Optional[torch.Tensor], activation: str = "none",
+                    want_x: bool = True, want_weight: bool = True, want_bias: bool = True):
+    """Gradients of ``linear_train_forward``: -> (x_bar, weight_bar, bias_bar), None where not wanted, in the tensors' type; the
+    residual's gradient is y_bar.  No floating point atomics: the same bits on every run."""
+    dtype, code, m, n, k = _linear_shapes(x, weight, activation)
+    shape = x.shape[:-1] + (n,)
+    if y_bar.shape != shape or (dact is not None and dact.shape != shape):
+        raise ValueError(f"linear_backward: y_bar and dact must be {tuple(shape)}")
+    if (dact is None) != (code == 0):
+        raise ValueError("linear_backward: dact (from linear_train_forward) is needed exactly when there is an activation")
+    x2, w2, g2 = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight"), _matrix(y_bar, m, n, x, "y_bar")
+    d2 = None if dact is None else _matrix(dact, m, n, x, "dact")
+    ldg, ldd = _ld(g2), 0 if d2 is None else _ld(d2)
+    lib = _lib.load()
+    new = lambda *s: torch.empty(*s, dtype=x.dtype, device=x.device)
+    x_bar = new(x.shape) if want_x else None
+    w_bar = new(n, k) if (want_weight or want_bias) else None
+    b_bar = new(n) if want_bias else None
+    with torch.cuda.device(x.device):
+        stream = _lib.stream_handle()
+        if want_x:
+            nbytes = lib.nrh_linear_workspace_bytes(1, dtype, m, n, k)
+            ws = _workspace(nbytes, x.device)
+            _lib.check(lib.nrh_linear_backward_data(dtype, _vp(g2), ldg, _vp(d2), ldd, code, _vp(w2), _ld(w2), m, n, k, _vp(x_bar), k,
+                                                    _vp(ws), nbytes, stream), "nrh_linear_backward_data")
+        if w_bar is not None:
+            nbytes = lib.nrh_linear_workspace_bytes(2, dtype, m, n, k)
+            ws = _workspace(nbytes, x.device)
+            _lib.check(lib.nrh_linear_backward_weight(dtype, _vp(g2), ldg, _vp(d2), ldd, code, _vp(x2), _ld(x2), m, n, k, _vp(w_bar), k,
+                                                      _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
+    return x_bar, (w_bar if want_weight else None), b_bar
+
+
+def _index(index, like, what):
+    if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64) or index.device != like.device:
+        raise ValueError(f"{what}: the index must be an int32 or int64 tensor on {like.device}")
+    return index.contiguous(), 64 if index.dtype == torch.int64 else 32
+
+
+def embedding(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * table[index]``: table [v, d], index int32 / int64 of any shape -> [..., d] in the table's type (product in float32,
+    one rounding).  An index outside [0, v) - a padded slot - gives a row of zeros and no gradient; there is no host check."""
+    dtype = _layer_input(table, "table")
+    if table.dim() != 2 or 0 in table.shape:
+        raise ValueError(f"embedding: table must be [v, d] with v, d >= 1, got {tuple(table.shape)}")
+    v, d = table.shape
+    idx, bits = _index(index, table, "embedding")
+    t2 = _matrix(table, v, d, table, "table")
+    rows = torch.empty(index.shape + (d,), dtype=table.dtype, device=table.device)
+    with torch.cuda.device(table.device):
+        _lib.check(_lib.load().nrh_embedding_forward(dtype, _vp(t2), _ld(t2), v, d, _vp(idx), bits, idx.numel(), float(scale), _vp(rows), d,
+                                                     _lib.stream_handle()), "nrh_embedding_forward")
+    return rows
+
+
+def embedding_backward(rows_bar: torch.Tensor, index: torch.Tensor, num_rows: int, scale: float = 1.0) -> torch.Tensor:
+    """Gradient of ``embedding`` with respect to its table: [num_rows, d], row r = scale * the sum of rows_bar over the tokens with
+    index r (float32 sums over tokens in their order, one rounding; zeros where there is none).  Tokens are sorted by index, nothing is
+    added atomically: the same bits on every run."""
+    dtype = _layer_input(rows_bar, "rows_bar")
+    if rows_bar.dim() < 1 or rows_bar.shape[:-1] != index.shape or rows_bar.shape[-1] < 1 or num_rows < 1:
+        raise ValueError(f"embedding_backward: rows_bar {tuple(rows_bar.shape)} does not fit index {tuple(index.shape)}, num_rows {num_rows}")
+    d = rows_bar.shape[-1]
+    idx, bits = _index(index, rows_bar, "embedding_backward")
+    n = idx.numel()
+    g2 = _matrix(rows_bar, n, d, rows_bar, "rows_bar")
+    out = torch.empty(num_rows, d, dtype=rows_bar.dtype, device=rows_bar.device)
+    lib = _lib.load()
+    with torch.cuda.device(rows_bar.device):
+        nbytes = lib.nrh_embedding_backward_workspace_bytes(n, num_rows, d)
+        ws = _workspace(nbytes, rows_bar.device)
+        _lib.check(lib.nrh_embedding_backward(dtype, _vp(g2), _ld(g2), _vp(idx), bits, n, num_rows, d, float(scale), _vp(out), d, _vp(ws),
+                                              nbytes, _lib.stream_handle()), "nrh_embedding_backward")
+    return out
