@@ -1850,6 +1850,11 @@ static int layer_result(int rc, const char* who) {
   return NRH_OK;
 }
 
+// act' is kept in float32 beside float16, in float16 beside bfloat16, and as a mask of the tensors' type for ReLU
+static bool dact_off_element(const void* p, int dtype, int act) {
+  return ((uintptr_t)p % (dtype == 0 || (dtype == 1 && act != nrhlin::RELU) ? 4 : 2)) != 0;
+}
+
 static bool off_element(const void* p, int dtype) { return ((uintptr_t)p % (dtype == 0 ? 4 : 2)) != 0; }
 
 static int linear_sizes(const char* who, int dtype, int act, long long m, long long n, long long k) {
@@ -1878,7 +1883,7 @@ int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, l
   if (ldx < k || ldw < k || ldy < n || (residual && ldr < n)) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
   if (activation == nrhlin::SOFTPLUS && !(beta > 0.0f && beta < 1e30f)) return fail(NRH_E_INVALID, "%s: softplus needs a positive beta", who);
   if (off_element(x, dtype) || off_element(w, dtype) || off_element(y, dtype) || off_element(bias, dtype) || off_element(residual, dtype) ||
-      off_element(dact, dtype))
+      dact_off_element(dact, dtype, activation))
     return fail(NRH_E_INVALID, "%s: a pointer is not aligned to its element", who);
   nrhlin::Call c = {};
   c.op = nrhlin::FORWARD;
@@ -1906,7 +1911,7 @@ static int linear_backward(int op, const char* who, int dtype, const void* ybar,
   if (m > 0 && (activation == nrhlin::NONE) != (dact == nullptr))
     return fail(NRH_E_INVALID, "%s: the saved derivative is needed exactly when there is an activation", who);
   if (ldyb < n || (dact && ldd < n) || ldother < k || ldo < k) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
-  if (off_element(ybar, dtype) || off_element(dact, dtype) || off_element(other, dtype) || off_element(out, dtype) || off_element(bias_bar, dtype))
+  if (off_element(ybar, dtype) || dact_off_element(dact, dtype, activation) || off_element(other, dtype) || off_element(out, dtype) || off_element(bias_bar, dtype))
     return fail(NRH_E_INVALID, "%s: a pointer is not aligned to its element", who);
   nrhlin::Call c = {};
   c.op = op;

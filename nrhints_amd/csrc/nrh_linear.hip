@@ -2,21 +2,26 @@
 //   zbar = ybar act'(z),   xbar = zbar W,   Wbar = zbar^T x,   bbar = sum_rows zbar.
 // float32, float16 and bfloat16 tensors; sums, bias, activation and residual in float32, one rounding to the tensor's type.
 //
-// All three products are  out[i, j] = sum_r A(i, r) B(j, r)  (nrh_layers.h) on one tiled kernel: a workgroup of four waves owns a
-// (64 NI) x (64 NJ) tile of the output and walks the reduction in steps of BK.  An operand's next step travels through registers
-// (global loads issued before the products of the current one) into LDS rows of BK values of the reduction, whatever its layout in
-// memory - reduction contiguous (ROWS) or tile axis contiguous (COLS: the 8 x V block a thread loads is transposed by indexing its
-// registers).  act' is applied on the way: zbar is never stored.
+// All three products are  out[i, j] = sum_r A(i, r) B(j, r)  (nrh_layers.h) on one tiled kernel: a workgroup of WI x WJ waves owns a
+// (32 NI WI) x (32 NJ WJ) tile of the output and walks the reduction in steps of BK, double-buffered in LDS.  The next step travels
+// through registers: loaded one step ahead, written to LDS beside the products of the current step, one barrier per step.
+// A chunk is 8 consecutive elements of a row in memory, whichever way the row runs:
+//   * ROWS (reduction contiguous): LDS rows of BK values per tile row; a lane's MFMA operand - 8 values of the reduction - is one
+//     ds_read_b128.
+//   * COLS (tile axis contiguous): LDS rows of the tile axis per value of the reduction; the operand is two ds_read_b64_tr_b16, which
+//     transpose 4 x 16 blocks on the way to the registers.
+// Both are swizzled by 16- or 64-byte groups so that neither the writes nor the reads of a wave meet in a bank.
+// act' is applied on the way to LDS: zbar is never stored.
 //   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' is rounded to the type once, as every operand of a 16-bit
-//     product is; for NONE and RELU it is exact.
+//     product is; for NONE and RELU it is exact.  act' itself is kept wider than the type (float32 beside float16, float16 beside
+//     bfloat16: 11 bits against 8), so that this one rounding is the only one.
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
 //     is scaled.  Infinities, NaN and values that round up to infinity make the parts NaN: a tile whose sums are not all finite is
 //     computed again with v_mfma_f32_32x32x2_f32, so its results are those of float32 arithmetic.
-// The MFMA's A role is played by the j operand: a lane then holds 16 values of ONE output row.  Its LDS rows are stored permuted (row
-// j = 16 h + 4 q + s of a block of 32 at 8 q + 4 h + s), which makes those 16 values consecutive columns.
-// LDS rows are padded by 16 B: 16 lanes reading the same 16-byte column of 16 rows meet 16 different bank groups.
+// The MFMA's A role is played by the j operand, its rows permuted (column j = 16 h + 4 q + s of a block of 32 is MFMA row
+// 8 q + 4 h + s): a lane then holds 16 consecutive columns of ONE output row.
 // A small output with a long reduction (every weight gradient) is split over the reduction; float32 partial tiles are joined in a
 // fixed order by reduce_kernel, so results do not depend on the order of execution.
 #include <hip/hip_runtime.h>
@@ -25,26 +30,94 @@
 
 namespace nrhlin {
 
-typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef long long ll;
 
 enum Src { ROWS = 0, COLS = 1 };
+enum Deriv { PLAIN = 0, SMOOTH = 1, MASK = 2 };      // A as it is, times act', or kept where act' > 0 (RELU)
 
-template <typename T> struct Ty;
-template <> struct Ty<float> { static constexpr int BK = 32, PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; };
-template <> struct Ty<_Float16> { static constexpr int BK = 64, PLANES = 1; typedef _Float16 L; typedef f16x8 L8; };
-template <> struct Ty<__bf16> { static constexpr int BK = 64, PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; };
+template <typename T> struct Ty;                    // BK, planes, LDS element, type act' is kept in
+template <> struct Ty<float> { static constexpr int BK = 32, PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; typedef float D; };
+template <> struct Ty<_Float16> { static constexpr int BK = 64, PLANES = 1; typedef _Float16 L; typedef f16x8 L8; typedef float D; };
+template <> struct Ty<__bf16> { static constexpr int BK = 64, PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; typedef _Float16 D; };
+
+template <bool C, typename A, typename B> struct Pick { typedef A type; };
+template <typename A, typename B> struct Pick<false, A, B> { typedef B type; };
+
+// 8 consecutive elements from any element-aligned address (global memory takes unaligned vector loads), as 32-bit words
+template <typename X> struct Chunk {
+  static constexpr int W = 2 * sizeof(X);
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const X* p) {
+    typedef uint32_t V2 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t V4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef typename Pick<sizeof(X) == 4, V4, V2>::type V;
+#pragma unroll
+    for (int h = 0; h < W; h += 4) {
+      const V x = *(const V*)((const uint32_t*)p + h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[h + e] = x[e];
+    }
+  }
+  // the first n (1 .. 8) of them and zeros, from the 8 that END with the n-th; n <= 0: zeros, from `safe`
+  __device__ __forceinline__ void load_last(const X* p, ll n, const X* safe) {
+    const int k = n >= 8 ? 0 : (n <= 0 ? 8 : 8 - (int)n);
+    load(k == 8 ? safe : p - k);
+    constexpr int PER = 4 / sizeof(X);                 // elements per word
+#pragma unroll
+    for (int step = 8; step >= PER; step /= 2) {
+      const bool on = (k & step) != 0;
+      const int by = step / PER;
+#pragma unroll
+      for (int e = 0; e < W; ++e) w[e] = on ? (e + by < W ? w[e + by] : 0u) : w[e];
+    }
+    if (PER == 2) {
+      const bool on = (k & 1) != 0;
+#pragma unroll
+      for (int e = 0; e < W; ++e) w[e] = on ? (w[e] >> 16 | (e + 1 < W ? w[e + 1] << 16 : 0u)) : w[e];
+    }
+  }
+  // the same one by one, for tensors too small to hold 8 elements before the end
+  __device__ __forceinline__ void load_single(const X* p, ll n) {
+#pragma unroll
+    for (int e = 0; e < W; ++e) w[e] = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) {
+        if (sizeof(X) == 4) w[e % W] = ((const uint32_t*)p)[e];
+        else w[(e / 2) % W] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
+      }
+  }
+  __device__ __forceinline__ void floats(float* x) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (sizeof(X) == 4) x[e] = __builtin_bit_cast(float, w[e]);
+      else {
+        typedef X X2 __attribute__((ext_vector_type(2)));
+        x[e] = (float)__builtin_bit_cast(X2, w[(e / 2) % W])[e & 1];
+      }
+    }
+  }
+};
+
+// two floats -> two 16-bit values in a word, round to nearest even (one v_cvt_pk)
+template <typename L> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  typedef float F2 __attribute__((ext_vector_type(2)));
+  typedef L L2 __attribute__((ext_vector_type(2)));
+  const F2 x = {a, b};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(x, L2));
+}
 
 struct Args {
-  const void *ip, *iq, *jp;        // A operand, its act' factor (or null), B operand
+  const void *ip, *iq, *jp;        // A operand, its act' (or null), B operand
   ll ild, iqld, jld;
   ll I, J, R;
-  int ivec, iqvec, jvec, ovec;     // rows start on vector boundaries: vector loads / stores allowed
-  int mask;                        // the factor is a mask (RELU)
+  int ovec;                        // out, residual, dact: rows start on vector boundaries
   int TI, TJ, S;                   // tiles, splits of the reduction
   ll chunk;                        // reduction per split, a multiple of BK
   void* out;
@@ -59,123 +132,49 @@ struct Args {
 };
 
 // ---- activation ------------------------------------------------------------------------------------------------------------
+// e^-a for a >= 0 on v_exp_f32 (2^x, 1 ulp), the argument a log2(e) in two parts: relative error 2^-23 up to a = 87, 0 beyond 150
+__device__ __forceinline__ float exp_minus(float a) {
+  a = fminf(a, 150.0f);
+  const float h = a * 1.44269502f;
+  const float l = fmaf(a, 1.92596299e-8f, fmaf(a, 1.44269502f, -h));
+  return __builtin_amdgcn_exp2f(-h) * fmaf(l, -0.693147182f, 1.0f);
+}
+
 // act(z) and act'(z); every exponential has a non-positive argument, so none overflows, and NaN passes through
 __device__ __forceinline__ float act_eval(int act, float beta, float z, float& d) {
   if (act == NONE) { d = 1.0f; return z; }
   if (act == RELU) { d = z > 0.0f ? 1.0f : 0.0f; return z < 0.0f ? 0.0f : z; }
   if (act == SOFTPLUS) {
-    const float e = expf(-fabsf(beta * z));
-    const float s = 1.0f / (1.0f + e);
-    d = z > 0.0f ? s : e * s;
+    const float e = exp_minus(fabsf(beta * z));
+    const float s = __builtin_amdgcn_rcpf(1.0f + e);
+    d = z != z ? z : (z > 0.0f ? s : e * s);
     return (z < 0.0f ? 0.0f : z) + log1pf(e) / beta;
   }
   if (act == GELU) {
     const float phi = 0.5f * erfcf(-0.70710678118654752f * z);      // erfc: no cancellation for negative z
-    d = phi + z * (0.3989422804014327f * expf(-0.5f * z * z));
+    d = phi + z * (0.3989422804014327f * exp_minus(0.5f * z * z));
     return z * phi;
   }
-  const float e = expf(-fabsf(z));
-  const float r = 1.0f / (1.0f + e);
+  const float e = exp_minus(fabsf(z));
+  const float r = __builtin_amdgcn_rcpf(1.0f + e);
   const float s = z < 0.0f ? e * r : r, c = z < 0.0f ? r : e * r;   // sigmoid(z), sigmoid(-z)
-  if (act == SIGMOID) { d = s * c; return z != z ? z : s; }
+  if (act == SIGMOID) { d = z != z ? z : s * c; return z != z ? z : s; }
   d = s * (1.0f + z * c);
   return z * s;
 }
 
-// ---- staging -----------------------------------------------------------------------------------------------------------------
-// One operand's step of the reduction: ROWN tile rows x BK values, held as NC groups of 8 consecutive reduction values per thread.
-template <typename T, int SRC, int ROWN> struct Stage {
-  static constexpr int BK = Ty<T>::BK, CH = BK / 8, NC = ROWN * CH / 256;
-  T v[NC][8];
-
-  static __device__ __forceinline__ int row(int tid, int u) {
-    if (SRC == ROWS) return (tid + 256 * u) / CH;
-    return CH == 4 ? (tid >> 2) * NC + u : ((tid >> 2) & 31) * NC + u;
-  }
-  static __device__ __forceinline__ int col(int tid, int u) {
-    if (SRC == ROWS) return (tid + 256 * u) % CH;
-    return CH == 4 ? (tid & 3) : (tid & 3) + 4 * (tid >> 7);
-  }
-  // tile rows a0 .. of n, reduction r0 .. of rn; rows past n repeat the last one (never stored), reduction past rn is zero
-  __device__ __forceinline__ void load(const T* __restrict__ p, ll ld, ll a0, ll n, ll r0, ll rn, bool vec, int tid) {
-    if (SRC == ROWS) {
-#pragma unroll
-      for (int u = 0; u < NC; ++u) {
-        ll a = a0 + row(tid, u);
-        a = a < n ? a : n - 1;
-        const ll r = r0 + 8 * col(tid, u);
-        const T* q = p + a * ld + r;
-        if (vec && r + 8 <= rn) {
-          if (sizeof(T) == 4) {
-            const f32x4 x = *(const f32x4*)q, y = *(const f32x4*)((const float*)q + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) { v[u][e] = (T)x[e]; v[u][4 + e] = (T)y[e]; }
-          } else {
-            const typename Ty<T>::L8 x = *(const typename Ty<T>::L8*)q;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[u][e] = (T)x[e];
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[u][e] = r + e < rn ? q[e] : (T)0.0f;
-        }
-      }
-    } else {
-      const ll a = a0 + row(tid, 0);
-      const ll r = r0 + 8 * col(tid, 0);
-      typedef T V __attribute__((ext_vector_type(NC > 1 ? NC : 2)));
-      if (NC > 1 && vec && a + NC <= n) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (r + e < rn) {
-            const V x = *(const V*)(p + (r + e) * ld + a);
-#pragma unroll
-            for (int u = 0; u < NC; ++u) v[u][e] = x[u];
-          } else {
-#pragma unroll
-            for (int u = 0; u < NC; ++u) v[u][e] = (T)0.0f;
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-          for (int u = 0; u < NC; ++u) {
-            const ll au = a + u < n ? a + u : n - 1;
-            v[u][e] = r + e < rn ? p[(r + e) * ld + au] : (T)0.0f;
-          }
-      }
-    }
+// ---- LDS ---------------------------------------------------------------------------------------------------------------------
+// byte offset of a chunk in one plane of an operand's tile (BA tile rows x BK values of the reduction)
+template <int SRC, int BA, int BK> struct Tile {
+  static constexpr int BYTES = BA * BK * 2;
+  // ROWS: row = tile row, c = chunk along the reduction.  Rows of 128 or 64 bytes; 16 rows x one c fill the 64 banks once.
+  // COLS: row = value of the reduction, c = chunk along the tile axis.  4 rows x one 64-byte group fill the banks once.
+  static __device__ __forceinline__ int at(int row, int c) {
+    if (SRC == ROWS) return row * BK * 2 + ((BK == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3)) << 4);
+    const int g = (c >> 2) ^ (BA == 64 ? (row >> 1) & 1 : row & 3);
+    return row * BA * 2 + (g << 6) + ((c & 3) << 4);
   }
 };
-
-// x -> three bfloat16 parts (PLANES = 3) or itself
-template <typename T> __device__ __forceinline__ void put8(const float* x, char* dst, int plane_bytes);
-template <> __device__ __forceinline__ void put8<float>(const float* x, char* dst, int plane_bytes) {
-  bf16x8 p0, p1, p2;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    p0[e] = (__bf16)x[e];
-    const float r1 = x[e] - (float)p0[e];
-    p1[e] = (__bf16)r1;
-    p2[e] = (__bf16)(r1 - (float)p1[e]);
-  }
-  *(bf16x8*)dst = p0;
-  *(bf16x8*)(dst + plane_bytes) = p1;
-  *(bf16x8*)(dst + 2 * plane_bytes) = p2;
-}
-template <> __device__ __forceinline__ void put8<_Float16>(const float* x, char* dst, int) {
-  f16x8 p;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) p[e] = (_Float16)x[e];
-  *(f16x8*)dst = p;
-}
-template <> __device__ __forceinline__ void put8<__bf16>(const float* x, char* dst, int) {
-  bf16x8 p;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) p[e] = (__bf16)x[e];
-  *(bf16x8*)dst = p;
-}
 
 __device__ __forceinline__ int perm32(int j) {      // column 16 h + 4 q + s of a block of 32 -> MFMA row 8 q + 4 h + s
   return (j & ~31) | (((j >> 2) & 3) << 3) | (((j >> 4) & 1) << 2) | (j & 3);
@@ -184,29 +183,124 @@ __device__ __forceinline__ int perm32(int j) {      // column 16 h + 4 q + s of 
 __device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
 
-template <typename T> __device__ __forceinline__ float times_act(float y, T q, int mask) {
-  return mask ? ((float)q > 0.0f ? y : 0.0f) : y * (float)q;
+// the lane's MFMA operand: tile rows 32 blk + (lane & 31), reduction 16 kk + 8 (lane >> 5) + 0..7.  PERM: the rows permuted (COLS; a
+// ROWS tile is stored permuted)
+template <typename L8, int SRC, int BA, int BK, bool PERM> __device__ __forceinline__ L8 fragment(const char* plane, int blk, int kk, int lane) {
+  if (SRC == ROWS) return *(const L8*)(plane + Tile<SRC, BA, BK>::at(blk * 32 + (lane & 31), 2 * kk + (lane >> 5)));
+  // ds_read_b64_tr_b16: lane s of 16 addresses 4 columns of one row; lane i receives column i of the four rows 4 s' .. 4 s' + 3
+  const int b = (lane >> 4) & 1, s = lane & 15, x = s & 3;
+  const int row = 16 * kk + 8 * (lane >> 5) + (s >> 2), col = PERM ? 16 * (x & 1) + 4 * (2 * b + (x >> 1)) : 16 * b + 4 * x;
+  const int off = row * BA * 2 + ((blk ^ (BA == 64 ? (row >> 1) & 1 : row & 3)) << 6) + col * 2;
+  typedef __attribute__((address_space(3))) i16x4 lds4;
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(plane + off));
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(plane + off + 4 * BA * 2));
+  return __builtin_bit_cast(L8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// bias, activation, residual of one output element; returns y and leaves act' in d
-template <typename T>
-__device__ __forceinline__ float finish(const Args& a, ll i, ll j, float z, float& d) {
-  if (a.bias) z += (float)((const T*)a.bias)[j];
-  float y = act_eval(a.act, a.beta, z, d);
-  if (a.res) y += (float)((const T*)a.res)[i * a.ldr + j];
-  return y;
-}
+// ---- staging -----------------------------------------------------------------------------------------------------------------
+template <typename T, int DM> struct Factor { typedef typename Ty<T>::D type; };
+template <typename T> struct Factor<T, MASK> { typedef T type; };
 
-template <typename T, int OP, int NI, int NJ>
-__global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
+// One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: the tensors may hold fewer than
+// 8 elements before an end (reductions shorter than 8, or a tiny tensor).
+template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> struct Stage {
+  typedef typename Factor<T, DM>::type Q;
+  typedef typename Ty<T>::L L;
+  static constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
+  typedef Tile<SRC, BA, BK> Tl;
+  Chunk<T> v[NC];
+  Chunk<Q> q[DM != PLAIN ? NC : 1];
+
+  // tile rows from a0 (of n), reduction from r0 (of rn; R in memory).  Rows past n repeat the last one and columns past n hold
+  // whatever follows in memory: neither reaches an output.  The reduction past rn is zero.  A step that lies inside the tensor takes
+  // addresses of one uniform base per chunk plus one 32-bit lane offset; at the edges every chunk is checked.
+  template <typename X> static __device__ __forceinline__ void fetch(Chunk<X>* c, const X* p, ll ld, ll a0, ll n, ll r0, ll rn, ll R, int tid) {
+    constexpr int ROW = SRC == ROWS ? CH : CW, STEP = NT / ROW;
+    if (a0 + BA <= n && r0 + BK <= rn && ld < (1 << 22)) {
+      const X* base = p + (SRC == ROWS ? a0 * ld + r0 : r0 * ld + a0);
+      const unsigned lane = (unsigned)(tid / ROW) * (unsigned)ld + 8 * (tid % ROW);
+#pragma unroll
+      for (int u = 0; u < NC; ++u) c[u].load(base + u * STEP * ld + lane);
+    } else {
+#pragma unroll
+      for (int u = 0; u < NC; ++u) {
+        const int row = tid / ROW + u * STEP, col = 8 * (tid % ROW);
+        ll a = a0 + (SRC == ROWS ? row : col);
+        const ll r = r0 + (SRC == ROWS ? col : row);
+        const X* at;
+        ll left;                                        // elements that may be taken from here
+        if (SRC == ROWS) {
+          a = a < n ? a : n - 1;
+          at = p + a * ld + r;
+          left = rn - r;
+        } else {
+          at = p + r * ld + a;
+          left = r < rn && a < n ? (R - 1 - r) * ld + n - a : 0;      // past the row's end lies the next row, up to the tensor's end
+        }
+        if (SINGLE) c[u].load_single(at, left);
+        else c[u].load_last(at, left, p);
+        __builtin_amdgcn_sched_barrier(0);               // one chunk after another: this is not the path to hold registers for
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const T* p, ll ld, const Q* pq, ll ldq, ll a0, ll n, ll r0, ll rn, ll R, int tid) {
+    fetch<T>(v, p, ld, a0, n, r0, rn, R, tid);
+    if (DM != PLAIN) fetch<Q>(q, pq, ldq, a0, n, r0, rn, R, tid);
+  }
+  // chunk u to LDS; SUMS: the chunk's 8 columns added up (COLS)
+  template <bool SUMS> __device__ __forceinline__ void put(int u, char* lds, float* sums, int tid) {
+    constexpr int ROW = SRC == ROWS ? CH : CW;
+    const int row = (tid + NT * u) / ROW, c = tid % ROW;
+    char* dst = lds + Tl::at(PERM && SRC == ROWS ? perm32(row) : row, c);
+    typedef uint32_t V __attribute__((ext_vector_type(4)));
+    if constexpr (PL == 1 && DM == PLAIN && !SUMS) {    // 16-bit, as it is
+      *(V*)dst = V{v[u].w[0], v[u].w[1], v[u].w[2], v[u].w[3]};
+      return;
+    }
+    float x[8], f[8];
+    v[u].floats(x);
+    if (DM != PLAIN) q[u].floats(f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (DM == SMOOTH) x[e] *= f[e];
+      if (DM == MASK) x[e] = f[e] > 0.0f ? x[e] : 0.0f;
+      if (SUMS) sums[e] += x[e];
+    }
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+      V y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[e] = pack2<L>(x[2 * e], x[2 * e + 1]);
+        if (PL == 3 && p < 2) {                         // the rest for the next bfloat16
+          x[2 * e] -= __builtin_bit_cast(float, y[e] << 16);
+          x[2 * e + 1] -= __builtin_bit_cast(float, y[e] & 0xffff0000u);
+        }
+      }
+      *(V*)(dst + p * Tl::BYTES) = y;
+    }
+  }
+};
+
+// ---- the tile kernel ---------------------------------------------------------------------------------------------------------
+template <typename T, int OP, int WI, int WJ, int NI, int NJ> struct Shape {
+  static constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
+  static constexpr int BUF = PL * (BI + BJ) * BK * 2;                               // one step
+  static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
+  static constexpr int EXACT = PL == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
+  static constexpr int SUMS = OP == BACK_WEIGHT ? NT * 8 * 4 : 0;
+  static constexpr int m1 = 2 * BUF > EPI ? 2 * BUF : EPI, m2 = EXACT > SUMS ? EXACT : SUMS, LDS = m1 > m2 ? m1 : m2;
+};
+
+template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, bool SINGLE>
+__global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
+  typedef Shape<T, OP, WI, WJ, NI, NJ> Sh;
   constexpr int SI = OP == BACK_WEIGHT ? COLS : ROWS, SJ = OP == FORWARD ? ROWS : COLS;
-  constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, BI = 64 * NI, BJ = 64 * NJ;
-  constexpr int PITCH = BK * 2 + 16, PLANE = (BI + BJ) * PITCH;
-  constexpr int EPITCH = 32 * NJ + 4, EPI = 4 * 32 * EPITCH * 4;
-  constexpr int EXACT = PL == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
-  constexpr int LDS = PL * PLANE > EPI ? (PL * PLANE > EXACT ? PL * PLANE : EXACT) : (EPI > EXACT ? EPI : EXACT);
+  constexpr int BK = Sh::BK, PL = Sh::PL, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
   typedef typename Ty<T>::L8 L8;
-  __shared__ __align__(16) char lds[LDS];
+  typedef Stage<T, SI, DM, false, BI, NT, SINGLE> StI;
+  typedef Stage<T, SJ, PLAIN, true, BJ, NT, SINGLE> StJ;
+  extern __shared__ __align__(16) char lds[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   // consecutive tiles (same A rows) go to one XCD: workgroups are dealt to the 8 XCDs in turn, and each has its own L2
@@ -219,83 +313,82 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
   const ll rbeg = s * a.chunk, rend = rbeg + a.chunk < a.R ? rbeg + a.chunk : a.R;
 
   const T* ip = (const T*)a.ip;
-  const T* iq = (const T*)a.iq;
+  const typename StI::Q* iq = (const typename StI::Q*)a.iq;
   const T* jp = (const T*)a.jp;
-  Stage<T, SI, BI> si, sq;
-  Stage<T, SJ, BJ> sj;
-  const bool scaled = OP != FORWARD && iq != nullptr;
-  const bool sums = OP == BACK_WEIGHT && a.bias_bar && tj == 0;
-  float bs[Stage<T, SI, BI>::NC] = {};
-
-  const int wi = wave >> 1, wj = wave & 1;
-  f32x16 acc[NI][NJ] = {};
+  StI si;
+  StJ sj;
+  float bs[8] = {};
   auto fill = [&](ll r) {
-    si.load(ip, a.ild, i0, a.I, r, rend, a.ivec, tid);
-    if (scaled) sq.load(iq, a.iqld, i0, a.I, r, rend, a.iqvec, tid);
-    sj.load(jp, a.jld, j0, a.J, r, rend, a.jvec, tid);
+    si.load(ip, a.ild, iq, a.iqld, i0, a.I, r, rend, a.R, tid);
+    sj.load(jp, a.jld, (const typename StJ::Q*)nullptr, 0, j0, a.J, r, rend, a.R, tid);
   };
-  fill(rbeg);
-  for (ll r = rbeg; r < rend; r += BK) {
+  auto put = [&](int buf) {
+    char* b = lds + buf * Sh::BUF;
+#pragma unroll
+    for (int u = 0; u < StI::NC; ++u) si.template put<OP == BACK_WEIGHT>(u, b, bs, tid);
+#pragma unroll
+    for (int u = 0; u < StJ::NC; ++u) sj.template put<false>(u, b + PL * StI::Tl::BYTES, nullptr, tid);
+  };
+
+  const int wi = wave / WJ, wj = wave % WJ;
+  f32x16 acc[NI][NJ] = {};
+  auto products = [&](int buf, int kk) {
+    const char* bi = lds + buf * Sh::BUF;
+    const char* bj = bi + PL * StI::Tl::BYTES;
+    L8 fi[NI][PL], fj[NJ][PL];
+#pragma unroll
+    for (int p = 0; p < PL; ++p) {
+#pragma unroll
+      for (int b = 0; b < NI; ++b) fi[b][p] = fragment<L8, SI, BI, BK, false>(bi + p * StI::Tl::BYTES, wi * NI + b, kk, lane);
+#pragma unroll
+      for (int b = 0; b < NJ; ++b) fj[b][p] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b, kk, lane);
+    }
+#pragma unroll
+    for (int sum = PL - 1; sum >= 0; --sum)            // the small products first
+#pragma unroll
+      for (int p = sum; p >= 0; --p)
+#pragma unroll
+        for (int x = 0; x < NI; ++x)
+#pragma unroll
+          for (int y = 0; y < NJ; ++y) acc[x][y] = mfma(fj[y][p], fi[x][sum - p], acc[x][y]);
+  };
+  if (rbeg < rend) {
+    fill(rbeg);
+    put(0);
+    if (rbeg + BK < rend) fill(rbeg + BK);
     __syncthreads();
+    int buf = 0;
+    for (ll r = rbeg; r + BK < rend; r += BK) {
+      products(buf, 0);
+      put(buf ^ 1);
+      if (r + 2 * BK < rend) fill(r + 2 * BK);
 #pragma unroll
-    for (int u = 0; u < si.NC; ++u) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = scaled ? times_act((float)si.v[u][e], sq.v[u][e], a.mask) : (float)si.v[u][e];
-      if (sums) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) bs[u] += x[e];
-      }
-      put8<T>(x, lds + si.row(tid, u) * PITCH + si.col(tid, u) * 16, PLANE);
+      for (int kk = 1; kk < KK; ++kk) products(buf, kk);
+      __syncthreads();
+      buf ^= 1;
     }
 #pragma unroll
-    for (int u = 0; u < sj.NC; ++u) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = (float)sj.v[u][e];
-      put8<T>(x, lds + (BI + perm32(sj.row(tid, u))) * PITCH + sj.col(tid, u) * 16, PLANE);
-    }
-    __syncthreads();
-    if (r + BK < rend) fill(r + BK);
-#pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      L8 fi[NI][PL], fj[NJ][PL];
-      const int off = (2 * kk + (lane >> 5)) * 16;
-#pragma unroll
-      for (int p = 0; p < PL; ++p) {
-#pragma unroll
-        for (int b = 0; b < NI; ++b) fi[b][p] = *(const L8*)(lds + p * PLANE + ((wi * NI + b) * 32 + (lane & 31)) * PITCH + off);
-#pragma unroll
-        for (int b = 0; b < NJ; ++b) fj[b][p] = *(const L8*)(lds + p * PLANE + (BI + (wj * NJ + b) * 32 + (lane & 31)) * PITCH + off);
-      }
-#pragma unroll
-      for (int sum = PL - 1; sum >= 0; --sum)          // the small products first
-#pragma unroll
-        for (int p = sum; p >= 0; --p)
-#pragma unroll
-          for (int bi = 0; bi < NI; ++bi)
-#pragma unroll
-            for (int bj = 0; bj < NJ; ++bj) acc[bi][bj] = mfma(fj[bj][p], fi[bi][sum - p], acc[bi][bj]);
-    }
+    for (int kk = 0; kk < KK; ++kk) products(buf, kk);
   }
 
   if (PL == 3) {
     int bad = 0;
 #pragma unroll
-    for (int bi = 0; bi < NI; ++bi)
+    for (int x = 0; x < NI; ++x)
 #pragma unroll
-      for (int bj = 0; bj < NJ; ++bj)
+      for (int y = 0; y < NJ; ++y)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) bad |= !(fabsf(acc[bi][bj][e]) < __builtin_huge_valf());
+        for (int e = 0; e < 16; ++e)
+          bad |= !(fabsf(acc[x][y][e]) < __builtin_huge_valf()) && j0 + (wj * NJ + y) * 32 + 16 * (lane >> 5) + e < a.J;
     if (__syncthreads_or(bad)) {                       // float32 products: rows of BK + 1 floats, two values of the reduction per MFMA
       float* fl = (float*)lds;
 #pragma unroll
-      for (int bi = 0; bi < NI; ++bi)
+      for (int x = 0; x < NI; ++x)
 #pragma unroll
-        for (int bj = 0; bj < NJ; ++bj) acc[bi][bj] = f32x16{};
+        for (int y = 0; y < NJ; ++y) acc[x][y] = f32x16{};
       for (ll r = rbeg; r < rend; r += BK) {
         __syncthreads();
-        for (int q = tid; q < (BI + BJ) * BK; q += 256) {
+        for (int q = tid; q < (BI + BJ) * BK; q += NT) {
           const int rr = q % BK, row = q / BK;
           const ll rg = r + rr;
           float x = 0.0f;
@@ -304,7 +397,10 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
               ll i = i0 + row;
               i = i < a.I ? i : a.I - 1;
               x = (float)ip[SI == ROWS ? i * a.ild + rg : rg * a.ild + i];
-              if (scaled) x = times_act(x, iq[SI == ROWS ? i * a.iqld + rg : rg * a.iqld + i], a.mask);
+              if (DM != PLAIN) {
+                const float d = (float)iq[SI == ROWS ? i * a.iqld + rg : rg * a.iqld + i];
+                x = DM == MASK ? (d > 0.0f ? x : 0.0f) : x * d;
+              }
             } else {
               ll j = j0 + row - BI;
               j = j < a.J ? j : a.J - 1;
@@ -321,9 +417,9 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
 #pragma unroll
           for (int b = 0; b < NJ; ++b) fj[b] = fl[(BI + (wj * NJ + b) * 32 + (lane & 31)) * (BK + 1) + kk + (lane >> 5)];
 #pragma unroll
-          for (int bi = 0; bi < NI; ++bi)
+          for (int x = 0; x < NI; ++x)
 #pragma unroll
-            for (int bj = 0; bj < NJ; ++bj) acc[bi][bj] = __builtin_amdgcn_mfma_f32_32x32x2f32(fj[bj], fi[bi], acc[bi][bj], 0, 0, 0);
+            for (int y = 0; y < NJ; ++y) acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x2f32(fj[y], fi[x], acc[x][y], 0, 0, 0);
         }
       }
     }
@@ -331,6 +427,7 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
 
   // the tile leaves through LDS, 32 rows of a wave at a time: a lane then finishes 4 consecutive columns and rows are stored whole
   float* ep = (float*)lds + wave * 32 * EPITCH;
+  typedef typename Ty<T>::D D;
   T* out = (T*)a.out;
 #pragma unroll
   for (int bi = 0; bi < NI; ++bi) {
@@ -359,7 +456,9 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
         continue;
       }
       typedef T T4 __attribute__((ext_vector_type(4)));
-      T4 y4, d4;
+      typedef D D4 __attribute__((ext_vector_type(4)));
+      T4 y4, m4;
+      D4 d4;
       if (OP == FORWARD) {
         T4 r4 = {};
         const bool whole = a.ovec && j + 4 <= a.J;
@@ -372,7 +471,8 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
           float y = act_eval(a.act, a.beta, x, d);
           if (a.res) y += whole ? (float)r4[e] : (float)((const T*)a.res)[i * a.ldr + j + e];
           y4[e] = (T)y;
-          d4[e] = (T)d;
+          d4[e] = (D)d;
+          m4[e] = (T)d;
         }
       } else {
 #pragma unroll
@@ -380,32 +480,46 @@ __global__ __launch_bounds__(256, 2) void tile_kernel(const Args a) {
       }
       if (a.ovec && j + 4 <= a.J) {
         *(T4*)(out + i * a.ldo + j) = y4;
-        if (OP == FORWARD && a.dact) *(T4*)((T*)a.dact + i * a.J + j) = d4;
+        if (OP == FORWARD && a.dact) {
+          if (a.act == RELU) *(T4*)((T*)a.dact + i * a.J + j) = m4;
+          else *(D4*)((D*)a.dact + i * a.J + j) = d4;
+        }
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (j + e >= a.J) break;
           out[i * a.ldo + j + e] = y4[e];
-          if (OP == FORWARD && a.dact) ((T*)a.dact)[i * a.J + j + e] = d4[e];
+          if (OP == FORWARD && a.dact) {
+            if (a.act == RELU) ((T*)a.dact)[i * a.J + j + e] = m4[e];
+            else ((D*)a.dact)[i * a.J + j + e] = d4[e];
+          }
         }
       }
     }
   }
 
-  if (sums) {                                          // bbar: the CH threads that share a column
-    constexpr int NC = Stage<T, SI, BI>::NC, CH = BK / 8;
+  if (OP == BACK_WEIGHT && a.bias_bar && tj == 0) {    // bbar: the threads that share 8 columns
     float* fl = (float*)lds;
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < NC; ++u) fl[si.col(tid, u) * BI + si.row(tid, u)] = bs[u];
+    for (int e = 0; e < 8; ++e) fl[(tid / StI::CW) * BI + 8 * (tid % StI::CW) + e] = bs[e];
     __syncthreads();
     if (tid < BI && i0 + tid < a.I) {
       float x = 0.0f;
-      for (int c = 0; c < CH; ++c) x += fl[c * BI + tid];
+      for (int c = 0; c < NT / StI::CW; ++c) x += fl[c * BI + tid];
       if (a.part) a.part_bias[s * a.I + i0 + tid] = x;
       else ((T*)a.bias_bar)[i0 + tid] = (T)x;
     }
   }
+}
+
+// bias, activation, residual of one output element; returns y and leaves act' in d
+template <typename T>
+__device__ __forceinline__ float finish(const Args& a, ll i, ll j, float z, float& d) {
+  if (a.bias) z += (float)((const T*)a.bias)[j];
+  float y = act_eval(a.act, a.beta, z, d);
+  if (a.res) y += (float)((const T*)a.res)[i * a.ldr + j];
+  return y;
 }
 
 // joins the S partial outputs in order and finishes them like the tile kernel
@@ -427,22 +541,32 @@ __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
   float d = 0.0f;
   if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
   ((T*)a.out)[i * a.ldo + j] = (T)z;
-  if (OP == FORWARD && a.dact) ((T*)a.dact)[e] = (T)d;
+  if (OP == FORWARD && a.dact) {
+    if (a.act == RELU) ((T*)a.dact)[e] = (T)d;
+    else ((typename Ty<T>::D*)a.dact)[e] = (typename Ty<T>::D)d;
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 struct Plan {
-  int tile, S;
+  bool big, tiny;
+  int S;
   ll TI, TJ, chunk;
 };
+
+// tile edges of the large variant (the small one is 64 x 64)
+static constexpr int big_i(int dtype) { return dtype == F32 ? 256 : 128; }
+static constexpr int big_j(int dtype) { return 128; }
 
 // Which tile and how many splits of the reduction: 256 CUs want at least one workgroup each.
 static Plan plan(int dtype, ll I, ll J, ll R) {
   const int BK = dtype == F32 ? 32 : 64;
-  auto tiles = [&](int t) { return ((I + t - 1) / t) * ((J + t - 1) / t); };
+  auto tiles = [&](int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); };
   Plan p;
-  p.tile = tiles(128) >= 192 || (I >= 128 && J >= 128 && R >= 8192) ? 128 : 64;
-  const ll n = tiles(p.tile) < 1 ? 1 : tiles(p.tile);
+  p.tiny = R < 8 || I < 8 || J < 8;         // an operand may hold fewer than 8 elements before its end: loaded one by one
+  p.big = !p.tiny && (tiles(big_i(dtype), big_j(dtype)) >= 192 || (I >= 128 && J >= 128 && R >= 8192));
+  const int ti = p.big ? big_i(dtype) : 64, tj = p.big ? big_j(dtype) : 64;
+  const ll n = tiles(ti, tj) < 1 ? 1 : tiles(ti, tj);
   ll s = n >= 256 ? 1 : 512 / n, most = R / (4 * BK);
   s = s < most ? s : most;
   s = s < 1 ? 1 : (s > 512 ? 512 : s);
@@ -450,8 +574,8 @@ static Plan plan(int dtype, ll I, ll J, ll R) {
   if (p.chunk < BK) p.chunk = BK;                       // R = 0: the gradient of no rows, one pass over nothing
   p.S = (int)((R + p.chunk - 1) / p.chunk);
   if (p.S < 1) p.S = 1;
-  p.TI = (I + p.tile - 1) / p.tile;
-  p.TJ = (J + p.tile - 1) / p.tile;
+  p.TI = (I + ti - 1) / ti;
+  p.TJ = (J + tj - 1) / tj;
   return p;
 }
 
@@ -468,6 +592,28 @@ long long workspace_bytes(int op, int dtype, long long m, long long n, long long
   return p.S == 1 ? 0 : 4 * (ll)p.S * (I * J + (op == BACK_WEIGHT ? I : 0));
 }
 
+// more than 64 KB of LDS has to be asked for, once per kernel and device (idempotent: no lock)
+template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, bool SINGLE = false> static int start(const Args& a, unsigned grid, hipStream_t st) {
+  typedef Shape<T, OP, WI, WJ, NI, NJ> Sh;
+  static bool ready[64];
+  int dev = -1;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -2;
+  auto* kernel = tile_kernel<T, OP, DM, WI, WJ, NI, NJ, SINGLE>;
+  if (!ready[dev]) {
+    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS) != hipSuccess) return -2;
+    ready[dev] = true;
+  }
+  kernel<<<dim3(grid), Sh::NT, Sh::LDS, st>>>(a);
+  return 0;
+}
+
+template <typename T, int OP, int DM> static int start_tile(const Args& a, bool big, bool tiny, unsigned grid, hipStream_t st) {
+  if (tiny) return start<T, OP, DM, 2, 2, 1, 1, true>(a, grid, st);
+  if (!big) return start<T, OP, DM, 2, 2, 1, 1>(a, grid, st);
+  if constexpr (sizeof(T) == 4) return start<T, OP, DM, 4, 2, 2, 2>(a, grid, st);
+  else return start<T, OP, DM, 2, 2, 2, 2>(a, grid, st);
+}
+
 template <typename T, int OP>
 static int run(const Call& c, hipStream_t st) {
   Args a = {};
@@ -476,18 +622,13 @@ static int run(const Call& c, hipStream_t st) {
   const ll need = workspace_bytes(OP, c.dtype, c.m, c.n, c.k);
   if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
   const int es = (int)sizeof(T);
-  // 16-byte loads of 8 reduction values (two for float32); the transposing loads are narrower
-  auto aligned = [&](const void* q, ll ld, int bytes) { return q && ((uintptr_t)q % bytes) == 0 && (ld * es) % bytes == 0 ? 1 : 0; };
+  auto aligned = [&](const void* q, ll ld, int bytes) { return ((uintptr_t)q % bytes) == 0 && ld % 4 == 0; };
   a.ip = OP == FORWARD ? c.x : c.ybar;
   a.ild = OP == FORWARD ? c.ldx : c.ldyb;
   a.iq = OP == FORWARD ? nullptr : c.dact;
   a.iqld = c.ldd;
   a.jp = OP == BACK_WEIGHT ? c.x : c.w;
   a.jld = OP == BACK_WEIGHT ? c.ldx : c.ldw;
-  a.ivec = aligned(a.ip, a.ild, 16);
-  a.iqvec = aligned(a.iq, a.iqld, 16);
-  a.jvec = aligned(a.jp, a.jld, 16);
-  a.mask = c.act == RELU;
   a.TI = (int)p.TI;
   a.TJ = (int)p.TJ;
   a.S = p.S;
@@ -501,14 +642,18 @@ static int run(const Call& c, hipStream_t st) {
   a.act = c.act;
   a.beta = c.beta;
   a.bias_bar = c.bias_bar;
-  a.ovec = aligned(a.out, a.ldo, 4 * es) && (!a.res || aligned(a.res, a.ldr, 4 * es)) && (!a.dact || aligned(a.dact, a.J, 4 * es));
+  const int ds = c.act == RELU ? es : (int)sizeof(typename Ty<T>::D);
+  a.ovec = aligned(a.out, a.ldo, 4 * es) && (!a.res || aligned(a.res, a.ldr, 4 * es)) && (!a.dact || aligned(a.dact, a.J, 4 * ds));
   if (p.S > 1) {
     a.part = (float*)c.ws;
     a.part_bias = a.part + (ll)p.S * a.I * a.J;
   }
-  const dim3 grid((unsigned)(p.TI * p.TJ * p.S));
-  if (p.tile == 128) tile_kernel<T, OP, 2, 2><<<grid, 256, 0, st>>>(a);
-  else tile_kernel<T, OP, 1, 1><<<grid, 256, 0, st>>>(a);
+  const unsigned grid = (unsigned)(p.TI * p.TJ * p.S);
+  int rc;
+  if constexpr (OP == FORWARD) rc = start_tile<T, OP, PLAIN>(a, p.big, p.tiny, grid, st);
+  else rc = c.act == NONE ? start_tile<T, OP, PLAIN>(a, p.big, p.tiny, grid, st) : (c.act == RELU ? start_tile<T, OP, MASK>(a, p.big, p.tiny, grid, st)
+                                                                                          : start_tile<T, OP, SMOOTH>(a, p.big, p.tiny, grid, st));
+  if (rc) return rc;
   if (p.S > 1) {
     const ll n = a.I * a.J + (a.bias_bar ? a.I : 0);
     reduce_kernel<T, OP><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(a);

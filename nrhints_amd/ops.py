@@ -299,13 +299,15 @@ def color_composite(color, weights, wsum, background=None, inside=None, grad=Non
 ACTIVATIONS = ("none", "relu", "softplus", "sigmoid", "silu", "gelu")
 _ACT = {name: code for code, name in enumerate(ACTIVATIONS)}
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+#: what act' is kept in between forward and backward (ReLU: a mask of the tensors' own type)
+_DACT = {torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
 
 
-def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str) -> torch.Tensor:
-    """``t`` as a [rows, cols] matrix of contiguous rows on ``like``'s device and of its type: a view where the strides allow it (a
-    column block of a wider buffer), else a copy."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{what}: expected a {like.dtype} tensor on {like.device}, got {getattr(t, 'dtype', type(t))} on {getattr(t, 'device', None)}")
+def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str, dtype=None) -> torch.Tensor:
+    """``t`` as a [rows, cols] matrix of contiguous rows on ``like``'s device and of its type (or ``dtype``): a view where the strides
+    allow it (a column block of a wider buffer), else a copy."""
+    if not isinstance(t, torch.Tensor) or t.dtype != (dtype or like.dtype) or t.device != like.device:
+        raise ValueError(f"{what}: expected a {dtype or like.dtype} tensor on {like.device}, got {getattr(t, 'dtype', type(t))} on {getattr(t, 'device', None)}")
     if t.dim() != 2:
         t = t.reshape(rows, cols)
     if (t.stride(1) != 1 and cols > 1) or (t.stride(0) < cols and rows > 1):
@@ -358,7 +360,7 @@ def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
     r2 = None if residual is None else _matrix(residual, m, n, x, "residual")
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     keep = want_dact and code != 0 and not (code == 1 and residual is None)
-    dact = torch.empty(shape, dtype=x.dtype, device=x.device) if keep else None
+    dact = torch.empty(shape, dtype=x.dtype if code == 1 else _DACT[x.dtype], device=x.device) if keep else None
     lib = _lib.load()
     with torch.cuda.device(x.device):
         nbytes = lib.nrh_linear_workspace_bytes(0, dtype, m, n, k)
@@ -383,8 +385,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 def linear_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                          residual: Optional[torch.Tensor] = None, activation: str = "none",
                          beta: float = 100.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) in the tensors' type, None for
-    "none", and y itself for "relu" without a residual (do not change y in place before the backward then)."""
+    """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) - float32 beside
+    float32 and float16, float16 beside bfloat16 -, None for "none", a mask for "relu": y itself where there is no residual (do not change
+    y in place before the backward then)."""
     return _linear_forward(x, weight, bias, residual, activation, beta, True)
 
 
@@ -399,7 +402,7 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
     if (dact is None) != (code == 0):
         raise ValueError("linear_backward: dact (from linear_train_forward) is needed exactly when there is an activation")
     x2, w2, g2 = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight"), _matrix(y_bar, m, n, x, "y_bar")
-    d2 = None if dact is None else _matrix(dact, m, n, x, "dact")
+    d2 = None if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else _DACT[x.dtype])
     ldg, ldd = _ld(g2), 0 if d2 is None else _ld(d2)
     lib = _lib.load()
     new = lambda *s: torch.empty(*s, dtype=x.dtype, device=x.device)

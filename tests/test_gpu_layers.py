@@ -5,7 +5,7 @@ Tolerances are bounds, computed element by element from the operands (u32 = 2^-2
     bfloat16 split of float32 operands, whose left-out products are below 2 u32 |a b|, bias and residual);
   * an activation is evaluated to 8 u32 of its value and passes the argument's error on with its Lipschitz constant;
   * every output is rounded once: uT |value| (float16: at least half a subnormal step, 2^-25); in the backward of a 16-bit type
-    act' and ybar act' are rounded once each (not for "none" and "relu", where they are exact).
+    ybar act' is rounded once (not for "none" and "relu", where it is exact), and act' once to the wider type it is kept in.
 ReLU's gradient is tested on operands whose sums are exact in float32, so that the sign of an argument is no matter of rounding."""
 import math
 
@@ -78,7 +78,8 @@ def check_linear(x, w, b, r, yb, act, beta, train=True):
         # (|d| + 1: act' is a sum of terms of size up to 1 + |z| that may cancel)
         ed = curve * ez + 16 * U32 * (1.0 + (z.abs() if act in ("silu", "gelu") else 0.0)) if act not in ("none", "relu") else torch.zeros_like(z)
         exact_zb = dtype == torch.float32 or act in ("none", "relu")
-        ezb = YB.abs() * (ed * (1 + 4 * ut(dtype)) + (0.0 if exact_zb else 1.0) * (2.01 * ut(dtype) * d.abs() + 2 * tiny(dtype)))
+        kept = {torch.float32: 0.0, torch.float16: 0.0, torch.bfloat16: ut(torch.float16)}[dtype]      # the rounding of act'
+        ezb = YB.abs() * (ed * (1 + 4 * ut(dtype)) + (0.0 if exact_zb else 1.0) * ((1.01 * ut(dtype) + kept) * d.abs() + 2.0 ** -25))
         ezb = ezb + (U32 * (YB * d).abs() if not act == "none" else 0.0) + (0.0 if exact_zb else tiny(dtype))
         zb = (YB * d).abs()
         ex = ezb @ W.abs() + (n + 8) * U32 * (zb @ W.abs()) + 1.01 * ut(dtype) * grads[0].abs() + tiny(dtype)
