@@ -64,6 +64,16 @@ template <typename X> struct Chunk {
       for (int e = 0; e < 4; ++e) w[h + e] = x[e];
     }
   }
+  __device__ __forceinline__ void load_16(const X* p) {      // 16 bytes: 8 elements of 16 bits, 4 of 32
+    typedef uint32_t V2 __attribute__((ext_vector_type(4), aligned(2)));
+    typedef uint32_t V4 __attribute__((ext_vector_type(4), aligned(4)));
+    typedef typename Pick<sizeof(X) == 4, V4, V2>::type V;
+    const V x = *(const V*)p;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = x[e];
+#pragma unroll
+    for (int e = 4; e < W; ++e) w[e] = 0;
+  }
   // the first n (1 .. 8) of them and zeros, from the 8 that END with the n-th; n <= 0: zeros, from `safe`
   __device__ __forceinline__ void load_last(const X* p, ll n, const X* safe) {
     const int k = n >= 8 ? 0 : (n <= 0 ? 8 : 8 - (int)n);
@@ -117,7 +127,6 @@ struct Args {
   const void *ip, *iq, *jp;        // A operand, its act' (or null), B operand
   ll ild, iqld, jld;
   ll I, J, R;
-  int ovec;                        // out, residual, dact: rows start on vector boundaries
   int TI, TJ, S;                   // tiles, splits of the reduction
   ll chunk;                        // reduction per split, a multiple of BK
   void* out;
@@ -282,11 +291,105 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> s
   }
 };
 
+// ---- results -----------------------------------------------------------------------------------------------------------------
+// bias, activation, residual of one output element; returns y and leaves act' in d
+template <typename T>
+__device__ __forceinline__ float finish(const Args& a, ll i, ll j, float z, float& d) {
+  if (a.bias) z += (float)((const T*)a.bias)[j];
+  float y = act_eval(a.act, a.beta, z, d);
+  if (a.res) y += (float)((const T*)a.res)[i * a.ldr + j];
+  return y;
+}
+
+template <typename T> __device__ __forceinline__ void keep(const Args& a, ll e, float d) {
+  if (a.act == RELU) ((T*)a.dact)[e] = (T)d;
+  else ((typename Ty<T>::D*)a.dact)[e] = (typename Ty<T>::D)d;
+}
+
+// N floats -> N elements of type X at any element-aligned address, 16 bytes per store
+template <typename X, int N> __device__ __forceinline__ void store(X* p, const float* x) {
+  typedef uint32_t V2 __attribute__((ext_vector_type(4), aligned(2)));
+  typedef uint32_t V4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef typename Pick<sizeof(X) == 4, V4, V2>::type V;
+  constexpr int PER = 16 / sizeof(X);
+  static_assert(N % 4 == 0, "");
+  if constexpr (N < PER) {                             // 4 16-bit elements
+    typedef uint32_t H __attribute__((ext_vector_type(2), aligned(2)));
+    *(H*)p = H{pack2<X>(x[0], x[1]), pack2<X>(x[2], x[3])};
+  } else {
+#pragma unroll
+    for (int h = 0; h < N; h += PER) {
+      V y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(X) == 4) y[e] = __builtin_bit_cast(uint32_t, x[h + e]);
+        else y[e] = pack2<X>(x[h + 2 * e], x[h + 2 * e + 1]);
+      }
+      *(V*)(p + h) = y;
+    }
+  }
+}
+
+// ROWS_ x COLS_ finished values of one wave, wholly inside the output.  MODE: an activation (FORWARD), STORE (as they are) or RAW
+// (float32 partial sums).
+enum Mode { STORE = 16, RAW = 17 };
+template <typename T, int ROWS_, int COLS_, int EPITCH, int MODE>
+__device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const float* ep, ll i0, ll j0, int lane) {
+  constexpr int C = MODE == RAW || sizeof(T) == 4 ? 4 : 8, LPR = COLS_ / C, RPI = 64 / LPR, UN = 4;
+  static_assert(ROWS_ % (RPI * UN) == 0 || ROWS_ / RPI < UN, "");
+  const int col = C * (lane % LPR), row0 = lane / LPR;
+  const ll j = j0 + col;
+  float b[C];
+#pragma unroll
+  for (int e = 0; e < C; ++e) b[e] = 0.0f;
+  if (MODE < STORE && a.bias) {
+#pragma unroll
+    for (int e = 0; e < C; ++e) b[e] = (float)((const T*)a.bias)[j + e];
+  }
+  constexpr int IT = ROWS_ / RPI, U = IT < UN ? IT : UN;
+#pragma unroll 1
+  for (int it = 0; it < IT; it += U) {
+    Chunk<T> r[U];                                     // C elements of the residual (float32: the first half)
+    if constexpr (MODE < STORE) if (a.res) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) r[u].load_16((const T*)a.res + (i0 + row0 + (it + u) * RPI) * a.ldr + j);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int row = row0 + (it + u) * RPI;
+      const ll i = i0 + row;
+      float z[C], d[C], f[8];
+#pragma unroll
+      for (int h = 0; h < C; h += 4) {
+        const f32x4 x = *(const f32x4*)(ep + row * EPITCH + col + h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[h + e] = x[e];
+      }
+      if constexpr (MODE == RAW) store<float, C>((float*)out + i * ldo + j, z);
+      else {
+        if constexpr (MODE < STORE) {
+          if (a.res) r[u].floats(f);
+#pragma unroll
+          for (int e = 0; e < C; ++e) {
+            z[e] = act_eval(MODE, a.beta, z[e] + b[e], d[e]);
+            if (a.res) z[e] += f[e];
+          }
+          if (a.dact && MODE != NONE) {
+            if constexpr (MODE == RELU) store<T, C>((T*)a.dact + i * a.J + j, d);
+            else store<typename Ty<T>::D, C>((typename Ty<T>::D*)a.dact + i * a.J + j, d);
+          }
+        }
+        store<T, C>((T*)out + i * ldo + j, z);
+      }
+    }
+  }
+}
+
 // ---- the tile kernel ---------------------------------------------------------------------------------------------------------
 template <typename T, int OP, int WI, int WJ, int NI, int NJ> struct Shape {
   static constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
   static constexpr int BUF = PL * (BI + BJ) * BK * 2;                               // one step
-  static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
+  static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * NI * EPITCH * 4;  // the tile on its way out
   static constexpr int EXACT = PL == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
   static constexpr int SUMS = OP == BACK_WEIGHT ? NT * 8 * 4 : 0;
   static constexpr int m1 = 2 * BUF > EPI ? 2 * BUF : EPI, m2 = EXACT > SUMS ? EXACT : SUMS, LDS = m1 > m2 ? m1 : m2;
@@ -425,76 +528,41 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
     }
   }
 
-  // the tile leaves through LDS, 32 rows of a wave at a time: a lane then finishes 4 consecutive columns and rows are stored whole
-  float* ep = (float*)lds + wave * 32 * EPITCH;
-  typedef typename Ty<T>::D D;
-  T* out = (T*)a.out;
+  // the tile leaves through LDS: a lane then finishes 16 bytes of a row, and rows are stored in whole cache lines
+  float* ep = (float*)lds + wave * 32 * NI * EPITCH;
+  __syncthreads();
 #pragma unroll
-  for (int bi = 0; bi < NI; ++bi) {
-    __syncthreads();
+  for (int x = 0; x < NI; ++x)
 #pragma unroll
-    for (int bj = 0; bj < NJ; ++bj)
+    for (int y = 0; y < NJ; ++y)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        f32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = acc[bi][bj][4 * q + e];
-        *(f32x4*)(ep + (lane & 31) * EPITCH + bj * 32 + 16 * (lane >> 5) + 4 * q) = x;
-      }
-    __syncthreads();
-    constexpr int LPR = 8 * NJ;                        // lanes per row
-    for (int it = 0; it < 32 * LPR / 64; ++it) {
-      const int row = it * (64 / LPR) + lane / LPR, cc = 4 * (lane % LPR);
-      const ll i = i0 + (wi * NI + bi) * 32 + row, j = j0 + wj * NJ * 32 + cc;
+      for (int q = 0; q < 4; ++q)
+        *(f32x4*)(ep + (x * 32 + (lane & 31)) * EPITCH + y * 32 + 16 * (lane >> 5) + 4 * q) =
+            f32x4{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]};
+  __syncthreads();
+  const ll iw = i0 + wi * NI * 32, jw = j0 + wj * NJ * 32;
+  if (i0 + BI <= a.I && j0 + BJ <= a.J) {
+    if (a.part) emit<T, 32 * NI, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, lane);
+    else if (OP != FORWARD) emit<T, 32 * NI, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else if (a.act == NONE) emit<T, 32 * NI, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else if (a.act == RELU) emit<T, 32 * NI, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else if (a.act == SOFTPLUS) emit<T, 32 * NI, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else if (a.act == SIGMOID) emit<T, 32 * NI, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else if (a.act == SILU) emit<T, 32 * NI, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, lane);
+    else emit<T, 32 * NI, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, lane);
+  } else {                                             // a tile at an edge: one element per lane
+    for (int e = lane; e < 32 * NI * 32 * NJ; e += 64) {
+      const int row = e / (32 * NJ), col = e % (32 * NJ);
+      const ll i = iw + row, j = jw + col;
       if (i >= a.I || j >= a.J) continue;
-      const f32x4 z = *(const f32x4*)(ep + row * EPITCH + cc);
+      float z = ep[row * EPITCH + col], d;
       if (a.part) {
-        float* o = a.part + (s * a.I + i) * a.J + j;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (j + e < a.J) o[e] = z[e];
+        a.part[(s * a.I + i) * a.J + j] = z;
         continue;
       }
-      typedef T T4 __attribute__((ext_vector_type(4)));
-      typedef D D4 __attribute__((ext_vector_type(4)));
-      T4 y4, m4;
-      D4 d4;
-      if (OP == FORWARD) {
-        T4 r4 = {};
-        const bool whole = a.ovec && j + 4 <= a.J;
-        if (a.res && whole) r4 = *(const T4*)((const T*)a.res + i * a.ldr + j);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (j + e >= a.J) break;
-          float d, x = z[e];
-          if (a.bias) x += (float)((const T*)a.bias)[j + e];
-          float y = act_eval(a.act, a.beta, x, d);
-          if (a.res) y += whole ? (float)r4[e] : (float)((const T*)a.res)[i * a.ldr + j + e];
-          y4[e] = (T)y;
-          d4[e] = (D)d;
-          m4[e] = (T)d;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y4[e] = (T)z[e];
-      }
-      if (a.ovec && j + 4 <= a.J) {
-        *(T4*)(out + i * a.ldo + j) = y4;
-        if (OP == FORWARD && a.dact) {
-          if (a.act == RELU) *(T4*)((T*)a.dact + i * a.J + j) = m4;
-          else *(D4*)((D*)a.dact + i * a.J + j) = d4;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (j + e >= a.J) break;
-          out[i * a.ldo + j + e] = y4[e];
-          if (OP == FORWARD && a.dact) {
-            if (a.act == RELU) ((T*)a.dact)[i * a.J + j + e] = m4[e];
-            else ((D*)a.dact)[i * a.J + j + e] = d4[e];
-          }
-        }
-      }
+      if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
+      ((T*)a.out)[i * a.ldo + j] = (T)z;
+      if (OP == FORWARD && a.dact) keep<T>(a, i * a.J + j, d);
     }
   }
 
@@ -511,15 +579,6 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
       else ((T*)a.bias_bar)[i0 + tid] = (T)x;
     }
   }
-}
-
-// bias, activation, residual of one output element; returns y and leaves act' in d
-template <typename T>
-__device__ __forceinline__ float finish(const Args& a, ll i, ll j, float z, float& d) {
-  if (a.bias) z += (float)((const T*)a.bias)[j];
-  float y = act_eval(a.act, a.beta, z, d);
-  if (a.res) y += (float)((const T*)a.res)[i * a.ldr + j];
-  return y;
 }
 
 // joins the S partial outputs in order and finishes them like the tile kernel
@@ -541,10 +600,7 @@ __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
   float d = 0.0f;
   if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
   ((T*)a.out)[i * a.ldo + j] = (T)z;
-  if (OP == FORWARD && a.dact) {
-    if (a.act == RELU) ((T*)a.dact)[e] = (T)d;
-    else ((typename Ty<T>::D*)a.dact)[e] = (typename Ty<T>::D)d;
-  }
+  if (OP == FORWARD && a.dact) keep<T>(a, e, d);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
@@ -621,8 +677,6 @@ static int run(const Call& c, hipStream_t st) {
   const Plan p = plan(c.dtype, a.I, a.J, a.R);
   const ll need = workspace_bytes(OP, c.dtype, c.m, c.n, c.k);
   if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
-  const int es = (int)sizeof(T);
-  auto aligned = [&](const void* q, ll ld, int bytes) { return ((uintptr_t)q % bytes) == 0 && ld % 4 == 0; };
   a.ip = OP == FORWARD ? c.x : c.ybar;
   a.ild = OP == FORWARD ? c.ldx : c.ldyb;
   a.iq = OP == FORWARD ? nullptr : c.dact;
@@ -642,8 +696,6 @@ static int run(const Call& c, hipStream_t st) {
   a.act = c.act;
   a.beta = c.beta;
   a.bias_bar = c.bias_bar;
-  const int ds = c.act == RELU ? es : (int)sizeof(typename Ty<T>::D);
-  a.ovec = aligned(a.out, a.ldo, 4 * es) && (!a.res || aligned(a.res, a.ldr, 4 * es)) && (!a.dact || aligned(a.dact, a.J, 4 * ds));
   if (p.S > 1) {
     a.part = (float*)c.ws;
     a.part_bias = a.part + (ll)p.S * a.I * a.J;
