@@ -74,10 +74,8 @@ template <typename X> struct Chunk {
 #pragma unroll
     for (int e = 4; e < W; ++e) w[e] = 0;
   }
-  // the first n (1 .. 8) of them and zeros, from the 8 that END with the n-th; n <= 0: zeros, from `safe`
-  __device__ __forceinline__ void load_last(const X* p, ll n, const X* safe) {
-    const int k = n >= 8 ? 0 : (n <= 0 ? 8 : 8 - (int)n);
-    load(k == 8 ? safe : p - k);
+  // the 8 elements behind p moved down by k (0 .. 8): p + k .. and zeros
+  __device__ __forceinline__ void drop(int k) {
     constexpr int PER = 4 / sizeof(X);                 // elements per word
 #pragma unroll
     for (int step = 8; step >= PER; step /= 2) {
@@ -231,6 +229,7 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> s
 #pragma unroll
       for (int u = 0; u < NC; ++u) c[u].load(base + u * STEP * ld + lane);
     } else {
+      int gone[NC];                                     // a chunk at an end: the last 8 elements, and so many of them dropped
 #pragma unroll
       for (int u = 0; u < NC; ++u) {
         const int row = tid / ROW + u * STEP, col = 8 * (tid % ROW);
@@ -247,8 +246,18 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> s
           left = r < rn && a < n ? (R - 1 - r) * ld + n - a : 0;      // past the row's end lies the next row, up to the tensor's end
         }
         if (SINGLE) c[u].load_single(at, left);
-        else c[u].load_last(at, left, p);
-        __builtin_amdgcn_sched_barrier(0);               // one chunk after another: this is not the path to hold registers for
+        else {
+          gone[u] = left >= 8 ? 0 : (left <= 0 ? 8 : 8 - (int)left);
+          c[u].load(left <= 0 ? p : at - gone[u]);
+        }
+        __builtin_amdgcn_sched_barrier(0);               // addresses one after another: this is not the path to hold registers for
+      }
+      if (!SINGLE) {
+#pragma unroll
+        for (int u = 0; u < NC; ++u) {
+          c[u].drop(gone[u]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
     }
   }
@@ -551,10 +560,10 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
     else if (a.act == SILU) emit<T, 32 * NI, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, lane);
     else emit<T, 32 * NI, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, lane);
   } else {                                             // a tile at an edge: one element per lane
-    for (int e = lane; e < 32 * NI * 32 * NJ; e += 64) {
-      const int row = e / (32 * NJ), col = e % (32 * NJ);
+    const int rows = a.I - iw < 32 * NI ? (int)(a.I - iw) : 32 * NI, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
+    for (int e = lane; e < rows * cols && cols > 0; e += 64) {
+      const int row = e / cols, col = e % cols;
       const ll i = iw + row, j = jw + col;
-      if (i >= a.I || j >= a.J) continue;
       float z = ep[row * EPITCH + col], d;
       if (a.part) {
         a.part[(s * a.I + i) * a.J + j] = z;
@@ -578,6 +587,52 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
       if (a.part) a.part_bias[s * a.I + i0 + tid] = x;
       else ((T*)a.bias_bar)[i0 + tid] = (T)x;
     }
+  }
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------------------------------
+// FORWARD for at most 8 rows of x: one wave per column of the output reads its row of W once, 16 bytes per lane, against all rows of
+// x (float32 FMA), and adds up over the wave.  Bound by reading W; x stays in the caches.
+template <typename T, int M>
+__global__ __launch_bounds__(256) void few_kernel(const Args a) {
+  constexpr int C = 16 / sizeof(T);
+  const int lane = threadIdx.x & 63;
+  const ll j = (ll)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (j >= a.J) return;
+  const T* w = (const T*)a.jp + j * a.jld;
+  const T* x = (const T*)a.ip;
+  float acc[M] = {};
+  const ll whole = a.R / C * C;
+#pragma unroll 2
+  for (ll r = lane * C; r < whole; r += 64 * C) {
+    Chunk<T> cw, cx;
+    float fw[8], fx[8];
+    cw.load_16(w + r);
+    cw.floats(fw);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      cx.load_16(x + m * a.ild + r);
+      cx.floats(fx);
+#pragma unroll
+      for (int e = 0; e < C; ++e) acc[m] = fmaf(fw[e], fx[e], acc[m]);
+    }
+  }
+  if (whole + lane < a.R) {
+    const float fw = (float)w[whole + lane];
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[m] = fmaf(fw, (float)x[m * a.ild + whole + lane], acc[m]);
+  }
+#pragma unroll
+  for (int m = 0; m < M; ++m)
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) acc[m] += __shfl_xor(acc[m], d);
+  float z = acc[0], d;
+#pragma unroll
+  for (int m = 1; m < M; ++m) z = lane == m ? acc[m] : z;
+  if (lane < M) {
+    z = finish<T>(a, lane, j, z, d);
+    ((T*)a.out)[lane * a.ldo + j] = (T)z;
+    if (a.dact) keep<T>(a, lane * a.J + j, d);
   }
 }
 
@@ -605,7 +660,7 @@ __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
 struct Plan {
-  bool big, tiny;
+  bool few, big, tiny;
   int S;
   ll TI, TJ, chunk;
 };
@@ -615,10 +670,13 @@ static constexpr int big_i(int dtype) { return dtype == F32 ? 256 : 128; }
 static constexpr int big_j(int dtype) { return 128; }
 
 // Which tile and how many splits of the reduction: 256 CUs want at least one workgroup each.
-static Plan plan(int dtype, ll I, ll J, ll R) {
+static Plan plan(int op, int dtype, ll I, ll J, ll R) {
   const int BK = dtype == F32 ? 32 : 64;
   auto tiles = [&](int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); };
-  Plan p;
+  Plan p = {};
+  p.S = 1;
+  p.few = op == FORWARD && I <= 8;
+  if (p.few) return p;
   p.tiny = R < 8 || I < 8 || J < 8;         // an operand may hold fewer than 8 elements before its end: loaded one by one
   p.big = !p.tiny && (tiles(big_i(dtype), big_j(dtype)) >= 192 || (I >= 128 && J >= 128 && R >= 8192));
   const int ti = p.big ? big_i(dtype) : 64, tj = p.big ? big_j(dtype) : 64;
@@ -644,7 +702,7 @@ static void shape(int op, ll m, ll n, ll k, ll& I, ll& J, ll& R) {
 long long workspace_bytes(int op, int dtype, long long m, long long n, long long k) {
   ll I, J, R;
   shape(op, m, n, k, I, J, R);
-  const Plan p = plan(dtype, I, J, R);
+  const Plan p = plan(op, dtype, I, J, R);
   return p.S == 1 ? 0 : 4 * (ll)p.S * (I * J + (op == BACK_WEIGHT ? I : 0));
 }
 
@@ -674,7 +732,7 @@ template <typename T, int OP>
 static int run(const Call& c, hipStream_t st) {
   Args a = {};
   shape(OP, c.m, c.n, c.k, a.I, a.J, a.R);
-  const Plan p = plan(c.dtype, a.I, a.J, a.R);
+  const Plan p = plan(OP, c.dtype, a.I, a.J, a.R);
   const ll need = workspace_bytes(OP, c.dtype, c.m, c.n, c.k);
   if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
   a.ip = OP == FORWARD ? c.x : c.ybar;
@@ -699,6 +757,22 @@ static int run(const Call& c, hipStream_t st) {
   if (p.S > 1) {
     a.part = (float*)c.ws;
     a.part_bias = a.part + (ll)p.S * a.I * a.J;
+  }
+  if constexpr (OP == FORWARD) {
+    if (p.few) {
+      const dim3 grid((unsigned)((a.J + 3) / 4));
+      switch (a.I) {
+        case 1: few_kernel<T, 1><<<grid, 256, 0, st>>>(a); break;
+        case 2: few_kernel<T, 2><<<grid, 256, 0, st>>>(a); break;
+        case 3: few_kernel<T, 3><<<grid, 256, 0, st>>>(a); break;
+        case 4: few_kernel<T, 4><<<grid, 256, 0, st>>>(a); break;
+        case 5: few_kernel<T, 5><<<grid, 256, 0, st>>>(a); break;
+        case 6: few_kernel<T, 6><<<grid, 256, 0, st>>>(a); break;
+        case 7: few_kernel<T, 7><<<grid, 256, 0, st>>>(a); break;
+        default: few_kernel<T, 8><<<grid, 256, 0, st>>>(a);
+      }
+      return hipGetLastError() == hipSuccess ? 0 : -2;
+    }
   }
   const unsigned grid = (unsigned)(p.TI * p.TJ * p.S);
   int rc;

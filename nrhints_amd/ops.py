@@ -303,28 +303,27 @@ _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _DACT = {torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
 
 
-def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str, dtype=None) -> torch.Tensor:
-    """``t`` as a [rows, cols] matrix of contiguous rows on ``like``'s device and of its type (or ``dtype``): a view where the strides
-    allow it (a column block of a wider buffer), else a copy."""
+def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str, dtype=None):
+    """``t`` as a [rows, cols] matrix of contiguous rows on ``like``'s device and of its type (or ``dtype``): -> (tensor, row stride), a
+    view where the strides allow it (a column block of a wider buffer), else a copy."""
     if not isinstance(t, torch.Tensor) or t.dtype != (dtype or like.dtype) or t.device != like.device:
         raise ValueError(f"{what}: expected a {dtype or like.dtype} tensor on {like.device}, got {getattr(t, 'dtype', type(t))} on {getattr(t, 'device', None)}")
+    if t.is_contiguous():
+        return t, cols
     if t.dim() != 2:
         t = t.reshape(rows, cols)
     if (t.stride(1) != 1 and cols > 1) or (t.stride(0) < cols and rows > 1):
         t = t.contiguous()
-    return t
-
-
-def _ld(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+    return t, (t.stride(0) if rows > 1 else cols)
 
 
 def _layer_input(x: torch.Tensor, what: str) -> int:
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError(f"{what}: expected a tensor on the GPU (there is no CPU path)")
-    if x.dtype not in _DTYPE:
+    code = _DTYPE.get(x.dtype)
+    if code is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16, got {x.dtype}")
-    return _DTYPE[x.dtype]
+    return code
 
 
 def _linear_shapes(x, weight, activation):
@@ -338,8 +337,37 @@ def _linear_shapes(x, weight, activation):
     return dtype, code, x.numel() // k, n, k
 
 
-def _workspace(nbytes: int, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+class _Here:
+    """``with _Here(device)``: the tensors' device current (the C entries launch on the current device) - nothing to do for the usual
+    case of one device - and its current stream as an integer."""
+    __slots__ = ("guard", "stream")
+
+    def __init__(self, device):
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        self.stream = torch.cuda.current_stream(device).cuda_stream
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+_WORKSPACE_BYTES = {}
+
+
+def _workspace(like: torch.Tensor, entry: str, *sizes: int):
+    """(workspace tensor | None, its bytes) of a C entry for these sizes; the size query is remembered, the memory is not."""
+    key = (entry,) + sizes
+    nbytes = _WORKSPACE_BYTES.get(key)
+    if nbytes is None:
+        if len(_WORKSPACE_BYTES) >= 4096:
+            _WORKSPACE_BYTES.clear()
+        nbytes = _WORKSPACE_BYTES[key] = getattr(_lib.load(), entry)(*sizes)
+    return (like.new_empty(nbytes, dtype=torch.uint8) if nbytes > 0 else None), nbytes
 
 
 def _vp(t):
@@ -350,24 +378,26 @@ def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
     dtype, code, m, n, k = _linear_shapes(x, weight, activation)
     if code == 2 and not 0.0 < float(beta) < 1e30:
         raise ValueError("linear: softplus needs a positive beta")
-    x2, w2 = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight")
+    (x2, ldx), (w2, ldw) = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight")
     shape = x.shape[:-1] + (n,)
-    if bias is not None and bias.shape != (n,):
-        raise ValueError(f"linear: bias must be [{n}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)} (it is not broadcast)")
-    b1 = None if bias is None else _matrix(bias.reshape(1, n), 1, n, x, "bias")
-    r2 = None if residual is None else _matrix(residual, m, n, x, "residual")
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
-    keep = want_dact and code != 0 and not (code == 1 and residual is None)
-    dact = torch.empty(shape, dtype=x.dtype if code == 1 else _DACT[x.dtype], device=x.device) if keep else None
-    lib = _lib.load()
-    with torch.cuda.device(x.device):
-        nbytes = lib.nrh_linear_workspace_bytes(0, dtype, m, n, k)
-        ws = _workspace(nbytes, x.device)
-        _lib.check(lib.nrh_linear_forward(dtype, _vp(x2), _ld(x2), _vp(w2), _ld(w2), _vp(b1), _vp(r2), 0 if r2 is None else _ld(r2), code,
-                                          float(beta), m, n, k, _vp(y), n, _vp(dact), _vp(ws), nbytes, _lib.stream_handle()),
-                   "nrh_linear_forward")
+    b1, r2, ldr = None, None, 0
+    if bias is not None:
+        if bias.shape != (n,):
+            raise ValueError(f"linear: bias must be [{n}], got {tuple(bias.shape)}")
+        b1, _ = _matrix(bias, 1, n, x, "bias")
+    if residual is not None:
+        if residual.shape != shape:
+            raise ValueError(f"linear: residual must have the output's shape {tuple(shape)}, got {tuple(residual.shape)} (it is not broadcast)")
+        r2, ldr = _matrix(residual, m, n, x, "residual")
+    y = x.new_empty(shape)
+    dact = None
+    if want_dact and code != 0 and not (code == 1 and residual is None):
+        dact = x.new_empty(shape, dtype=x.dtype if code == 1 else _DACT[x.dtype])
+    ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 0, dtype, m, n, k)
+    with _Here(x.device) as stream:
+        rc = _lib.load().nrh_linear_forward(dtype, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _vp(b1), _vp(r2), ldr, code, beta, m, n, k,
+                                            y.data_ptr(), n, _vp(dact), _vp(ws), nbytes, stream)
+    _lib.check(rc, "nrh_linear_forward")
     if want_dact and code == 1 and residual is None:
         dact = y           # ReLU: the output is positive exactly where the argument is
     return y, dact
@@ -401,26 +431,21 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
         raise ValueError(f"linear_backward: y_bar and dact must be {tuple(shape)}")
     if (dact is None) != (code == 0):
         raise ValueError("linear_backward: dact (from linear_train_forward) is needed exactly when there is an activation")
-    x2, w2, g2 = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight"), _matrix(y_bar, m, n, x, "y_bar")
-    d2 = None if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else _DACT[x.dtype])
-    ldg, ldd = _ld(g2), 0 if d2 is None else _ld(d2)
+    (x2, ldx), (w2, ldw), (g2, ldg) = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight"), _matrix(y_bar, m, n, x, "y_bar")
+    d2, ldd = (None, 0) if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else _DACT[x.dtype])
     lib = _lib.load()
-    new = lambda *s: torch.empty(*s, dtype=x.dtype, device=x.device)
-    x_bar = new(x.shape) if want_x else None
-    w_bar = new(n, k) if (want_weight or want_bias) else None
-    b_bar = new(n) if want_bias else None
-    with torch.cuda.device(x.device):
-        stream = _lib.stream_handle()
+    x_bar = x.new_empty(x.shape) if want_x else None
+    w_bar = x.new_empty((n, k)) if (want_weight or want_bias) else None
+    b_bar = x.new_empty((n,)) if want_bias else None
+    with _Here(x.device) as stream:
         if want_x:
-            nbytes = lib.nrh_linear_workspace_bytes(1, dtype, m, n, k)
-            ws = _workspace(nbytes, x.device)
-            _lib.check(lib.nrh_linear_backward_data(dtype, _vp(g2), ldg, _vp(d2), ldd, code, _vp(w2), _ld(w2), m, n, k, _vp(x_bar), k,
-                                                    _vp(ws), nbytes, stream), "nrh_linear_backward_data")
+            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 1, dtype, m, n, k)
+            _lib.check(lib.nrh_linear_backward_data(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, w2.data_ptr(), ldw, m, n, k,
+                                                    x_bar.data_ptr(), k, _vp(ws), nbytes, stream), "nrh_linear_backward_data")
         if w_bar is not None:
-            nbytes = lib.nrh_linear_workspace_bytes(2, dtype, m, n, k)
-            ws = _workspace(nbytes, x.device)
-            _lib.check(lib.nrh_linear_backward_weight(dtype, _vp(g2), ldg, _vp(d2), ldd, code, _vp(x2), _ld(x2), m, n, k, _vp(w_bar), k,
-                                                      _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
+            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 2, dtype, m, n, k)
+            _lib.check(lib.nrh_linear_backward_weight(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, x2.data_ptr(), ldx, m, n, k,
+                                                      w_bar.data_ptr(), k, _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
     return x_bar, (w_bar if want_weight else None), b_bar
 
 
@@ -438,11 +463,11 @@ def embedding(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> t
         raise ValueError(f"embedding: table must be [v, d] with v, d >= 1, got {tuple(table.shape)}")
     v, d = table.shape
     idx, bits = _index(index, table, "embedding")
-    t2 = _matrix(table, v, d, table, "table")
-    rows = torch.empty(index.shape + (d,), dtype=table.dtype, device=table.device)
-    with torch.cuda.device(table.device):
-        _lib.check(_lib.load().nrh_embedding_forward(dtype, _vp(t2), _ld(t2), v, d, _vp(idx), bits, idx.numel(), float(scale), _vp(rows), d,
-                                                     _lib.stream_handle()), "nrh_embedding_forward")
+    t2, ldt = _matrix(table, v, d, table, "table")
+    rows = table.new_empty(index.shape + (d,))
+    with _Here(table.device) as stream:
+        rc = _lib.load().nrh_embedding_forward(dtype, t2.data_ptr(), ldt, v, d, idx.data_ptr(), bits, idx.numel(), scale, rows.data_ptr(), d, stream)
+    _lib.check(rc, "nrh_embedding_forward")
     return rows
 
 
@@ -456,12 +481,11 @@ def embedding_backward(rows_bar: torch.Tensor, index: torch.Tensor, num_rows: in
     d = rows_bar.shape[-1]
     idx, bits = _index(index, rows_bar, "embedding_backward")
     n = idx.numel()
-    g2 = _matrix(rows_bar, n, d, rows_bar, "rows_bar")
-    out = torch.empty(num_rows, d, dtype=rows_bar.dtype, device=rows_bar.device)
-    lib = _lib.load()
-    with torch.cuda.device(rows_bar.device):
-        nbytes = lib.nrh_embedding_backward_workspace_bytes(n, num_rows, d)
-        ws = _workspace(nbytes, rows_bar.device)
-        _lib.check(lib.nrh_embedding_backward(dtype, _vp(g2), _ld(g2), _vp(idx), bits, n, num_rows, d, float(scale), _vp(out), d, _vp(ws),
-                                              nbytes, _lib.stream_handle()), "nrh_embedding_backward")
+    g2, ldg = _matrix(rows_bar, n, d, rows_bar, "rows_bar")
+    out = rows_bar.new_empty((num_rows, d))
+    ws, nbytes = _workspace(rows_bar, "nrh_embedding_backward_workspace_bytes", n, num_rows, d)
+    with _Here(rows_bar.device) as stream:
+        rc = _lib.load().nrh_embedding_backward(dtype, g2.data_ptr(), ldg, idx.data_ptr(), bits, n, num_rows, d, scale, out.data_ptr(), d, _vp(ws),
+                                                nbytes, stream)
+    _lib.check(rc, "nrh_embedding_backward")
     return out
