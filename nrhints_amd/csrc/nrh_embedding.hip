@@ -2,14 +2,17 @@
 //
 // The gradient sorts the tokens by index - stable, so a row's tokens stay in their order - and sums runs of equal index: no atomics on
 // floating point numbers, the same bits on every run, float32 sums, one rounding.
-//   sort      up to 2 048 tokens: bitonic in LDS, one launch; more: least significant digit first, 8 bits per pass (histogram of a
-//             tile of 2 048 tokens, scan per digit, ranked scatter), as many passes as the table's height has digits.
-//   zero      rows that no token names, found by bisection in the sorted keys (the others are written once, by the sums).
-//   sum       a group of lanes - one lane per 16 bytes of a row - walks 32 sorted tokens.  A run that begins and ends inside is
+//   low tables (at most 255 rows, partial tables of at most 8 MB): a workgroup sorts 512 tokens in LDS and sums them into its own [rows, d] partial table; a second
+//             launch adds the partial tables up (one workgroup of tokens: no second launch).
+//   others    sort: up to 2 048 tokens bitonic in LDS, one launch; more: least significant digit first, 8 bits per pass (histogram per
+//             tile of 1 024 tokens, ranked scatter; the scan between them is part of the scatter up to 64 tiles).
+//             sum: a group of lanes - one lane per 16 bytes of a row - walks 32 sorted tokens.  A run that begins and ends inside is
 //             written to the table; the first and the last run of a group may go on in its neighbours and are handed, as float32
-//             rows with their keys, to the next level, which does the same with 1/16 of the entries until one group is left.  A row
-//             named by every token and a table named once per row cost the same.
-// Both directions are bound by HBM: the tokens' rows are read once, the table's gradient is written once.
+//             rows with their keys, to the next level, which does the same, until one group is left.  A
+//             row named by every token and a table named once per row cost the same.  Rows that no token names are found by bisection
+//             in the sorted keys and cleared beside the first level: every row is written once.
+// Both directions are bound by HBM at large sizes (the tokens' rows are read once, the table's gradient is written once), by launches
+// at small ones.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "nrh_layers.h"
@@ -19,7 +22,7 @@ namespace nrhemb {
 typedef long long ll;
 typedef unsigned long long ull;
 constexpr unsigned NONE = 0xffffffffu;
-constexpr int TILE = 2048, SMALL = 2048, RUN = 32;
+constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 32, LOW = 255, LOW_TOKENS = 512;
 
 template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct Vec<T, 1> { typedef T type; };
@@ -91,7 +94,7 @@ struct Pass {
   ll n, v;
   const unsigned *keys_in, *perm_in;
   unsigned *keys_out, *perm_out;
-  unsigned *hist, *total;  // [256][tiles], [256]
+  unsigned *hist, *total;  // [tiles][256]; [256] (more than FOLD tiles: after scan_kernel)
   ll tiles;
 };
 
@@ -107,34 +110,35 @@ __global__ __launch_bounds__(256) void hist_kernel(const Pass p) {
     if (i < p.n) atomicAdd(&h[(pass_key(p, i) >> p.shift) & 255], 1u);      // counts: the order does not matter
   }
   __syncthreads();
-  p.hist[(ll)threadIdx.x * p.tiles + blockIdx.x] = h[threadIdx.x];
+  p.hist[(ll)blockIdx.x * 256 + threadIdx.x] = h[threadIdx.x];
 }
 
 // exclusive scan over 256 values, one per thread; buf [256]
 __device__ __forceinline__ unsigned scan256(unsigned x, unsigned* buf, unsigned& total) {
-  const int t = threadIdx.x;
-  __syncthreads();
-  buf[t] = x;
-  __syncthreads();
-  for (int d = 1; d < 256; d *= 2) {
-    const unsigned y = t >= d ? buf[t - d] : 0;
-    __syncthreads();
-    buf[t] += y;
-    __syncthreads();
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  unsigned in = x;                                       // inclusive within the wave
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const unsigned y = __shfl_up(in, d);
+    if (lane >= d) in += y;
   }
-  total = buf[255];
-  return buf[t] - x;
+  __syncthreads();
+  if (lane == 63) buf[wave] = in;
+  __syncthreads();
+  const unsigned w0 = buf[0], w1 = buf[1], w2 = buf[2];
+  total = w0 + w1 + w2 + buf[3];
+  return in - x + (wave > 0 ? w0 : 0) + (wave > 1 ? w1 : 0) + (wave > 2 ? w2 : 0);
 }
 
 __global__ __launch_bounds__(256) void scan_kernel(const Pass p) {
   __shared__ unsigned buf[256];
-  unsigned* h = p.hist + (ll)blockIdx.x * p.tiles;
+  unsigned* h = p.hist + blockIdx.x;                     // one digit
   unsigned carry = 0;
   for (ll b = 0; b < p.tiles; b += 256) {
     const ll i = b + threadIdx.x;
     unsigned total;
-    const unsigned ex = scan256(i < p.tiles ? h[i] : 0, buf, total);
-    if (i < p.tiles) h[i] = carry + ex;
+    const unsigned ex = scan256(i < p.tiles ? h[i * 256] : 0, buf, total);
+    if (i < p.tiles) h[i * 256] = carry + ex;
     carry += total;
   }
   if (threadIdx.x == 0) p.total[blockIdx.x] = carry;
@@ -145,18 +149,33 @@ __global__ __launch_bounds__(256) void scatter_kernel(const Pass p) {
   __shared__ unsigned cnt[4][256];
   __shared__ unsigned buf[256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
-  unsigned all;
-  const unsigned digit_base = scan256(p.total[tid], buf, all) + p.hist[(ll)tid * p.tiles + blockIdx.x];
-  __syncthreads();
-  volatile unsigned* mine = cnt[wave];
   const ll base = (ll)blockIdx.x * TILE + wave * (TILE / 4);
-  unsigned key[ROUNDS], rank[ROUNDS];
+  unsigned key[ROUNDS], from[ROUNDS], rank[ROUNDS];      // everything that is read, first
 #pragma unroll
   for (int r = 0; r < ROUNDS; ++r) {
     const ll i = base + r * 64 + lane;
-    const bool live = i < p.n;
-    key[r] = live ? pass_key(p, i) : 0;
+    key[r] = i < p.n ? pass_key(p, i) : 0;
+    from[r] = p.first ? (unsigned)i : (i < p.n ? p.perm_in[i] : 0);
+  }
+  for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+  unsigned all, before_me = 0, total = 0;                // of digit tid: in the tiles before this one, in all
+  if (p.tiles <= FOLD) {
+#pragma unroll 8
+    for (int t = 0; t < (int)p.tiles; ++t) {
+      const unsigned x = p.hist[t * 256 + tid];
+      before_me += t < (int)blockIdx.x ? x : 0;
+      total += x;
+    }
+  } else {
+    before_me = p.hist[(ll)blockIdx.x * 256 + tid];
+    total = p.total[tid];
+  }
+  const unsigned digit_base = scan256(total, buf, all) + before_me;
+  __syncthreads();
+  volatile unsigned* mine = cnt[wave];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const bool live = base + r * 64 + lane < p.n;
     const unsigned d = (key[r] >> p.shift) & 255;
     ull peers = __ballot(live);
 #pragma unroll
@@ -185,29 +204,12 @@ __global__ __launch_bounds__(256) void scatter_kernel(const Pass p) {
     if (i < p.n) {
       const unsigned to = cnt[wave][(key[r] >> p.shift) & 255] + rank[r];
       p.keys_out[to] = key[r];
-      p.perm_out[to] = p.first ? (unsigned)i : p.perm_in[i];
+      p.perm_out[to] = from[r];
     }
   }
 }
 
 // ---- sums --------------------------------------------------------------------------------------------------------------------
-// one wave per table row (and 64 V columns at a time): zeros where no sorted key equals the row
-template <typename T, int V>
-__global__ __launch_bounds__(256) void zero_kernel(const unsigned* __restrict__ keys, ll n, ll v, int cols, T* __restrict__ out, ll ldo) {
-  typedef typename Vec<T, V>::type VT;
-  for (ll row = (ll)blockIdx.x * 4 + (threadIdx.x >> 6); row < v; row += (ll)gridDim.x * 4) {
-    ll lo = 0, hi = n;
-    while (lo < hi) {
-      const ll mid = (lo + hi) / 2;
-      if (keys[mid] < (unsigned)row) lo = mid + 1;
-      else hi = mid;
-    }
-    if (lo < n && keys[lo] == (unsigned)row) continue;
-    const VT z = {};
-    for (int c = threadIdx.x & 63; c < cols; c += 64) *(VT*)(out + row * ldo + (ll)c * V) = z;
-  }
-}
-
 struct Level {
   const unsigned *keys, *perm;   // perm: first level only
   const void* rows;              // first level: T [.., ldr], else float [n][d]
@@ -218,16 +220,46 @@ struct Level {
   ll ldo;
   unsigned* next_keys;           // null: the last level
   float* next_rows;
+  int run;                       // entries per group
+  unsigned sum_blocks;           // first level: the workgroups after these clear rows
 };
+
+// 16 table rows per wave: zeros where no sorted key equals the row
+template <typename T, int V> __device__ __forceinline__ void clear_rows(const Level& a, ll wave, ll waves) {
+  typedef typename Vec<T, V>::type VT;
+  const int lane = threadIdx.x & 63;
+  for (ll r0 = wave * 16; r0 < a.v; r0 += waves * 16) {
+    bool clear = false;
+    if (lane < 16 && r0 + lane < a.v) {
+      const unsigned row = (unsigned)(r0 + lane);
+      ll lo = 0, hi = a.n;
+      while (lo < hi) {
+        const ll mid = (lo + hi) / 2;
+        if (a.keys[mid] < row) lo = mid + 1;
+        else hi = mid;
+      }
+      clear = !(lo < a.n && a.keys[lo] == row);
+    }
+    const VT z = {};
+    for (ull todo = __ballot(clear); todo; todo &= todo - 1) {
+      T* out = (T*)a.out + (r0 + __builtin_ctzll(todo)) * a.ldo;
+      for (int c = lane; c < a.cols; c += 64) *(VT*)(out + (ll)c * V) = z;
+    }
+  }
+}
 
 template <typename T, int V, bool FIRST>
 __global__ __launch_bounds__(256) void sum_kernel(const Level a) {
   typedef typename Vec<T, V>::type VT;
   typedef typename Vec<float, V>::type FT;
-  constexpr int BATCH = 8;
+  constexpr int BATCH = FIRST ? 8 : 16;
+  if (FIRST && blockIdx.x >= a.sum_blocks) {
+    if (blockIdx.y == 0) clear_rows<T, V>(a, (ll)(blockIdx.x - a.sum_blocks) * 4 + (threadIdx.x >> 6), (ll)(gridDim.x - a.sum_blocks) * 4);
+    return;
+  }
   const ll g = (ll)blockIdx.x * (256 / a.width) + threadIdx.x / a.width;
   const int c = blockIdx.y * a.width + threadIdx.x % a.width;
-  const ll beg = g * RUN, end = beg + RUN < a.n ? beg + RUN : a.n;
+  const ll beg = g * a.run, end = beg + a.run < a.n ? beg + a.run : a.n;
   if (beg >= a.n || c >= a.cols) return;
   const ll col = (ll)c * V;
   unsigned cur = NONE;
@@ -299,9 +331,130 @@ __global__ __launch_bounds__(256) void sum_kernel(const Level a) {
   }
 }
 
+// ---- low tables --------------------------------------------------------------------------------------------------------------
+struct Low {
+  const void* index;
+  int index64;
+  ll n, ldr, ldo;
+  int v, d, cols, width;
+  float scale;
+  const void* rows;
+  void* out;
+  float* part;                   // [workgroups][v][d]; null: one workgroup, which writes the table
+};
+
+// 512 tokens: counting sort by row in LDS (stable), then a group of lanes per row adds up its tokens
+template <typename T, int V>
+__global__ __launch_bounds__(256) void low_kernel(const Low a) {
+  typedef typename Vec<T, V>::type VT;
+  typedef typename Vec<float, V>::type FT;
+  constexpr int ROUNDS = LOW_TOKENS / 256, BATCH = 8;
+  __shared__ unsigned cnt[4][256];
+  __shared__ unsigned buf[256];
+  __shared__ unsigned start[257];
+  __shared__ unsigned short order[LOW_TOKENS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+  __syncthreads();
+  volatile unsigned* mine = cnt[wave];
+  const ll tok0 = (ll)blockIdx.x * LOW_TOKENS;
+  const int first = wave * (LOW_TOKENS / 4);
+  unsigned key[ROUNDS], rank[ROUNDS];
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r) {
+    const ll i = tok0 + first + r * 64 + lane;
+    const bool live = i < a.n;
+    key[r] = live ? key_of(a.index, a.index64, i, a.v) : 0;
+    ull peers = __ballot(live);
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const ull on = __ballot((key[r] >> b) & 1);
+      peers &= (key[r] >> b) & 1 ? on : ~on;
+    }
+    const unsigned before = (unsigned)__popcll(peers & ((1ull << lane) - 1));
+    if (live) {
+      const unsigned c = mine[key[r]];
+      rank[r] = c + before;
+      if (before == 0) mine[key[r]] = c + (unsigned)__popcll(peers);
+    }
+  }
+  __syncthreads();
+  unsigned own = 0, total;
+  for (int w = 0; w < 4; ++w) own += cnt[w][tid];
+  unsigned c = scan256(own, buf, total);
+  start[tid] = c;
+  if (tid == 255) start[256] = c + own;
+  for (int w = 0; w < 4; ++w) {
+    const unsigned x = cnt[w][tid];
+    cnt[w][tid] = c;
+    c += x;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ROUNDS; ++r)
+    if (tok0 + first + r * 64 + lane < a.n) order[cnt[wave][key[r]] + rank[r]] = (unsigned short)(first + r * 64 + lane);
+  __syncthreads();
+  const int per = 256 / a.width, g = tid / a.width;
+  for (int row = g; row < a.v; row += per) {
+    const unsigned beg = start[row], end = start[row + 1];
+    for (int col = tid % a.width; col < a.cols; col += a.width) {
+      float acc[V];
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+      for (unsigned e = beg; e < end; e += BATCH) {
+        VT x[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (e + b < end) x[b] = *(const VT*)((const T*)a.rows + (tok0 + order[e + b]) * a.ldr + (ll)col * V);
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          if (e + b < end) {
+#pragma unroll
+            for (int q = 0; q < V; ++q) acc[q] += at<T, V>(x[b], q);
+          }
+      }
+      if (a.part) {
+        FT y;
+#pragma unroll
+        for (int q = 0; q < V; ++q) put<float, V>(y, q, acc[q]);
+        *(FT*)(a.part + ((ll)blockIdx.x * a.v + row) * a.d + (ll)col * V) = y;
+      } else {
+        VT y;
+#pragma unroll
+        for (int q = 0; q < V; ++q) put<T, V>(y, q, a.scale * acc[q]);
+        *(VT*)((T*)a.out + row * a.ldo + (ll)col * V) = y;
+      }
+    }
+  }
+}
+
+// 64 elements of the table per workgroup, each as 16 sums over every 16th partial table, joined in order
+template <typename T>
+__global__ __launch_bounds__(1024) void low_join_kernel(const Low a, int parts) {
+  __shared__ float buf[16][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
+  const ll size = (ll)a.v * a.d, e = (ll)blockIdx.x * 64 + lane;
+  float x = 0.0f;
+  if (e < size) {
+#pragma unroll 8
+    for (int p = slice; p < parts; p += 16) x += a.part[p * size + e];
+  }
+  buf[slice][lane] = x;
+  __syncthreads();
+  if (slice == 0 && e < size) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) sum += buf[q][lane];
+    ((T*)a.out)[e / a.d * a.ldo + e % a.d] = (T)(a.scale * sum);
+  }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------------------------
 static ll align256(ll x) { return (x + 255) / 256 * 256; }
-static ll groups(ll n) { return (n + RUN - 1) / RUN; }
+static ll groups(ll n, int level) { return level == 0 ? (n + RUN0 - 1) / RUN0 : (n + RUN1 - 1) / RUN1; }
+static ll low_parts(ll n) { return (n + LOW_TOKENS - 1) / LOW_TOKENS; }
+// partial tables of up to 8 MB cost less to write and read (about 4 us) than the launches they save
+static bool low(ll n, ll v, ll d) { return v <= LOW && (low_parts(n) <= 1 || 4 * low_parts(n) * v * d <= (8 << 20)); }
 
 struct Layout {
   ll keys[2], perm[2], hist, total, lkeys[2], lrows[2], bytes;
@@ -321,7 +474,7 @@ static Layout layout(ll n, ll d) {
   }
   l.hist = take(1024 * ((n + TILE - 1) / TILE));
   l.total = take(1024);
-  const ll n1 = 2 * groups(n), n2 = 2 * groups(n1);
+  const ll n1 = 2 * groups(n, 0), n2 = 2 * groups(n1, 1);
   l.lkeys[0] = take(4 * n1);
   l.lrows[0] = take(4 * n1 * d);
   l.lkeys[1] = take(4 * n2);
@@ -331,8 +484,9 @@ static Layout layout(ll n, ll d) {
 }
 
 long long backward_workspace_bytes(long long n, long long v, long long d) {
-  (void)v;
-  return n <= 0 ? 0 : layout(n, d).bytes;
+  if (n <= 0) return 0;
+  if (low(n, v, d)) return low_parts(n) > 1 ? 4 * low_parts(n) * v * d : 0;
+  return layout(n, d).bytes;
 }
 
 // a grid's threads are counted in 32 bits: larger ranges loop
@@ -347,10 +501,34 @@ template <typename T, int V> static int forward_as(const Call& c, hipStream_t st
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
+template <typename T, int V> static int low_as(const Call& c, hipStream_t st) {
+  Low a;
+  a.index = c.index;
+  a.index64 = c.index64;
+  a.n = c.n;
+  a.ldr = c.lds;
+  a.ldo = c.ldd;
+  a.v = (int)c.v;
+  a.d = (int)c.d;
+  a.cols = (int)(c.d / V);
+  a.width = 1;
+  while (a.width < a.cols && a.width < 64) a.width *= 2;
+  a.scale = c.scale;
+  a.rows = c.src;
+  a.out = c.dst;
+  const ll parts = c.n > 0 ? low_parts(c.n) : 1;
+  a.part = parts > 1 ? (float*)c.ws : nullptr;
+  low_kernel<T, V><<<dim3((unsigned)parts), 256, 0, st>>>(a);
+  if (parts > 1) low_join_kernel<T><<<dim3((unsigned)((c.v * c.d + 63) / 64)), 1024, 0, st>>>(a, (int)parts);
+  return hipGetLastError() == hipSuccess ? 0 : -2;
+}
+
 template <typename T, int V> static int backward_as(const Call& c, hipStream_t st) {
+  const ll need = backward_workspace_bytes(c.n, c.v, c.d);
+  if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
+  if (low(c.n, c.v, c.d)) return low_as<T, V>(c, st);
   const int cols = (int)(c.d / V);
   const Layout l = layout(c.n, c.d);
-  if (c.n > 0 && (!c.ws || c.ws_bytes < l.bytes)) return -3;
   char* ws = (char*)c.ws;
   unsigned *keys[2], *perm[2];
   for (int b = 0; b < 2; ++b) {
@@ -378,13 +556,12 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
       p.keys_out = keys[cur];
       p.perm_out = perm[cur];
       hist_kernel<<<dim3((unsigned)p.tiles), 256, 0, st>>>(p);
-      scan_kernel<<<256, 256, 0, st>>>(p);
+      if (p.tiles > FOLD) scan_kernel<<<256, 256, 0, st>>>(p);
       scatter_kernel<<<dim3((unsigned)p.tiles), 256, 0, st>>>(p);
       cur = 1 - cur;
     }
     cur = 1 - cur;
   }
-  zero_kernel<T, V><<<blocks((c.v + 3) / 4), 256, 0, st>>>(keys[cur], c.n, c.v, cols, (T*)c.dst, c.ldd);
   Level a;
   a.v = c.v;
   a.d = (int)c.d;
@@ -395,10 +572,11 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
   a.out = c.dst;
   a.ldo = c.ldd;
   ll n = c.n;
-  for (int level = 0; n > 0; ++level) {
-    const ll g = groups(n);
-    const bool last = g == 1;
+  for (int level = 0; level == 0 || n > 0; ++level) {
+    const ll g = groups(n, level);
+    const bool last = g <= 1;
     a.n = n;
+    a.run = level == 0 ? RUN0 : RUN1;
     a.keys = level == 0 ? keys[cur] : (const unsigned*)(ws + l.lkeys[(level - 1) & 1]);
     a.perm = perm[cur];
     a.rows = level == 0 ? c.src : (const void*)(ws + l.lrows[(level - 1) & 1]);
@@ -406,7 +584,9 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
     a.next_keys = last ? nullptr : (unsigned*)(ws + l.lkeys[level & 1]);
     a.next_rows = (float*)(ws + l.lrows[level & 1]);
     const int per = 256 / a.width;
-    const dim3 grid((unsigned)((g + per - 1) / per), (unsigned)((cols + a.width - 1) / a.width));
+    a.sum_blocks = (unsigned)((g + per - 1) / per);
+    const ll clear = (c.v + 63) / 64 < (1 << 20) ? (c.v + 63) / 64 : (1 << 20);      // 16 rows per wave
+    const dim3 grid(a.sum_blocks + (level == 0 ? (unsigned)clear : 0u), (unsigned)((cols + a.width - 1) / a.width));
     if (level == 0) sum_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
     else sum_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
     n = last ? 0 : 2 * g;

@@ -344,7 +344,7 @@ class _Here:
 
     def __init__(self, device):
         self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-        self.stream = torch.cuda.current_stream(device).cuda_stream
+        self.stream = torch._C._cuda_getCurrentRawStream(device.index)      # current_stream(device).cuda_stream without the object
 
     def __enter__(self):
         if self.guard is not None:

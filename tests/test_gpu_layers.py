@@ -285,15 +285,19 @@ def check_embedding(v, d, n, dtype, spread, index_dtype, absent, scale, seed=0):
     assert rows.dtype == dtype and torch.equal(rows, want)
     gb = torch.randint(-8, 9, (n, d), generator=g, device="cuda").to(dtype)
     got = ops.embedding_backward(gb, idx, v, scale)
-    acc = torch.zeros(v, d, dtype=torch.float64, device="cuda").index_add_(0, safe, gb.double() * live[:, None])
+    acc = torch.zeros(v, d, dtype=torch.float64, device="cuda")
+    if spread == "one":
+        acc[v - 1] = (gb.double() * live[:, None]).sum(0)
+    else:
+        acc.index_add_(0, safe, gb.double() * live[:, None])
     assert float(acc.abs().max() if acc.numel() else 0) < 2 ** 24
     assert torch.equal(got, (acc.float() * scale).to(dtype)), (v, d, n)
 
 
 @pytest.mark.parametrize("dtype", DT, ids=IDS)
-@pytest.mark.parametrize("n", [0, 1, 2, 31, 32, 33, 64, 65, 1000, 2047, 2048, 2049, 5000, 70001])
+@pytest.mark.parametrize("n", [0, 1, 2, 31, 32, 33, 64, 65, 511, 512, 513, 1000, 2047, 2048, 2049, 5000, 70001, 140000])
 def test_embedding_tokens(n, dtype):
-    for v, d, spread in ((1, 3, "even"), (100, 12, "uneven"), (70000, 64, "even"), (300, 5, "one")):
+    for v, d, spread in ((1, 3, "even"), (100, 12, "uneven"), (70000, 64, "even"), (300, 5, "one"), (255, 260, "even"), (40, 9, "one")):
         check_embedding(v, d, n, dtype, spread, torch.int64 if n % 2 else torch.int32, 0.1, 1.0)
 
 

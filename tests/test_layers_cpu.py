@@ -40,7 +40,7 @@ def test_c_entries_refuse_bad_arguments():
                 dict(i=p + 4), dict(n=(1 << 30) + 1), dict(v=1 << 31), dict(t=p + 2)):
         assert emb(**bad) == -1, bad
     assert emb(n=0, i=None, o=None) == 0
-    assert lib.nrh_embedding_backward(0, p, 4, p, 64, 2, 3, 4, 1.0, p, 4, None, 0, None) == -3
+    assert lib.nrh_embedding_backward(0, p, 4, p, 64, 2, 300, 4, 1.0, p, 4, None, 0, None) == -3
     assert lib.nrh_embedding_backward(0, p, 4, p, 64, 2, 3, 4, 1.0, None, 4, None, 0, None) == -1
     assert lib.nrh_embedding_backward_workspace_bytes(-1, 3, 4) == -1 and lib.nrh_embedding_backward_workspace_bytes(0, 3, 4) == 0
 
