@@ -660,7 +660,7 @@ int nrh_sdf32_tables(const float* const* sdf_bias, const int* rows, const float*
  *   for a slot without a row: zeros.
  * nrh_embedding_backward   table_bar [v,d] = scale * sum of the rows_bar [n,d] of the tokens that name each row, every row written (zeros
  *   where no token names it); tokens are sorted by index and summed in a fixed order, without atomics: the same bits on every run. */
-long long nrh_linear_workspace_bytes(int op, int dtype, long long m, long long n, long long k);
+long long nrh_linear_workspace_bytes(int op, int dtype, int activation, long long m, long long n, long long k);
 int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* residual,
                        long long ldr, int activation, float beta, long long m, long long n, long long k, void* y, long long ldy,
                        void* dact, void* workspace, long long workspace_bytes, void* stream);

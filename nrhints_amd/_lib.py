@@ -234,7 +234,7 @@ def load():
     lib.nrh_sampler_fusion.restype = c_int
     lib.nrh_kernel_timing_read.argtypes = [POINTER(ctypes.c_double), POINTER(c_longlong)]
     L = c_longlong
-    lib.nrh_linear_workspace_bytes.argtypes = [c_int, c_int, L, L, L]
+    lib.nrh_linear_workspace_bytes.argtypes = [c_int, c_int, c_int, L, L, L]
     lib.nrh_linear_workspace_bytes.restype = L
     lib.nrh_linear_forward.argtypes = [c_int, P, L, P, L, P, P, L, c_int, c_float, L, L, L, P, L, P, P, L, P]
     lib.nrh_linear_backward_data.argtypes = [c_int, P, L, P, L, c_int, P, L, L, L, L, P, L, P, L, P]

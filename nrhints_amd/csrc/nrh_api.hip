@@ -1867,9 +1867,9 @@ static int linear_sizes(const char* who, int dtype, int act, long long m, long l
   return NRH_OK;
 }
 
-long long nrh_linear_workspace_bytes(int op, int dtype, long long m, long long n, long long k) {
-  if (op < 0 || op > 2 || dtype < 0 || dtype > 2 || m < 0 || n < 1 || k < 1) return -1;
-  return nrhlin::workspace_bytes(op, dtype, m, n, k);
+long long nrh_linear_workspace_bytes(int op, int dtype, int activation, long long m, long long n, long long k) {
+  if (op < 0 || op > 2 || dtype < 0 || dtype > 2 || activation < 0 || activation > 5 || m < 0 || n < 1 || k < 1) return -1;
+  return nrhlin::workspace_bytes(op, dtype, activation, m, n, k);
 }
 
 int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, long long ldw, const void* bias, const void* residual,

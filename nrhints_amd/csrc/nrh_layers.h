@@ -35,7 +35,7 @@ struct Call {
   void* ws;
   long long ws_bytes;
 };
-long long workspace_bytes(int op, int dtype, long long m, long long n, long long k);
+long long workspace_bytes(int op, int dtype, int act, long long m, long long n, long long k);
 int launch(const Call& c, hipStream_t st);     // 0 ok, -2 launch error, -3 workspace too small
 
 }  // namespace nrhlin

@@ -41,10 +41,10 @@ typedef long long ll;
 enum Src { ROWS = 0, COLS = 1 };
 enum Deriv { PLAIN = 0, SMOOTH = 1, MASK = 2 };      // A as it is, times act', or kept where act' > 0 (RELU)
 
-template <typename T> struct Ty;                    // BK, planes, LDS element, type act' is kept in
-template <> struct Ty<float> { static constexpr int BK = 32, PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; typedef float D; };
-template <> struct Ty<_Float16> { static constexpr int BK = 64, PLANES = 1; typedef _Float16 L; typedef f16x8 L8; typedef float D; };
-template <> struct Ty<__bf16> { static constexpr int BK = 64, PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; typedef _Float16 D; };
+template <typename T> struct Ty;                    // planes, LDS element, type act' is kept in
+template <> struct Ty<float> { static constexpr int PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; typedef float D; };
+template <> struct Ty<_Float16> { static constexpr int PLANES = 1; typedef _Float16 L; typedef f16x8 L8; typedef float D; };
+template <> struct Ty<__bf16> { static constexpr int PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; typedef _Float16 D; };
 
 template <bool C, typename A, typename B> struct Pick { typedef A type; };
 template <typename A, typename B> struct Pick<false, A, B> { typedef B type; };
@@ -100,6 +100,17 @@ template <typename X> struct Chunk {
         if (sizeof(X) == 4) w[e % W] = ((const uint32_t*)p)[e];
         else w[(e / 2) % W] |= (uint32_t)((const uint16_t*)p)[e] << (16 * (e & 1));
       }
+  }
+  __device__ __forceinline__ void pair(int e, float& a, float& b) const {      // elements 2 e and 2 e + 1
+    if constexpr (sizeof(X) == 4) {
+      a = __builtin_bit_cast(float, w[(2 * e) % W]);
+      b = __builtin_bit_cast(float, w[(2 * e + 1) % W]);
+    } else {
+      typedef X X2 __attribute__((ext_vector_type(2)));
+      const X2 t = __builtin_bit_cast(X2, w[e]);
+      a = (float)t[0];
+      b = (float)t[1];
+    }
   }
   __device__ __forceinline__ void floats(float* x) const {
 #pragma unroll
@@ -174,10 +185,10 @@ __device__ __forceinline__ float act_eval(int act, float beta, float z, float& d
 // byte offset of a chunk in one plane of an operand's tile (BA tile rows x BK values of the reduction)
 template <int SRC, int BA, int BK> struct Tile {
   static constexpr int BYTES = BA * BK * 2;
-  // ROWS: row = tile row, c = chunk along the reduction.  Rows of 128 or 64 bytes; 16 rows x one c fill the 64 banks once.
+  // ROWS: row = tile row, c = chunk along the reduction.  Rows of 128, 64 or 32 bytes; 16 rows x one c fill the 64 banks once.
   // COLS: row = value of the reduction, c = chunk along the tile axis.  4 rows x one 64-byte group fill the banks once.
   static __device__ __forceinline__ int at(int row, int c) {
-    if (SRC == ROWS) return row * BK * 2 + ((BK == 64 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3)) << 4);
+    if (SRC == ROWS) return row * BK * 2 + ((BK == 64 ? c ^ ((row >> 1) & 7) : (BK == 32 ? c ^ ((row >> 2) & 3) : c ^ ((row >> 3) & 1))) << 4);
     const int g = (c >> 2) ^ (BA == 64 ? (row >> 1) & 1 : row & 3);
     return row * BA * 2 + (g << 6) + ((c & 3) << 4);
   }
@@ -210,10 +221,10 @@ template <typename T> struct Factor<T, MASK> { typedef T type; };
 
 // One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: the tensors may hold fewer than
 // 8 elements before an end (reductions shorter than 8, or a tiny tensor).
-template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> struct Stage {
+template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool SINGLE> struct Stage {
   typedef typename Factor<T, DM>::type Q;
   typedef typename Ty<T>::L L;
-  static constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
+  static constexpr int PL = Ty<T>::PLANES, CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
   typedef Tile<SRC, BA, BK> Tl;
   Chunk<T> v[NC];
   Chunk<Q> q[DM != PLAIN ? NC : 1];
@@ -229,6 +240,8 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> s
 #pragma unroll
       for (int u = 0; u < NC; ++u) c[u].load(base + u * STEP * ld + lane);
     } else {
+      // (addresses are worked out here, every time: moved out of the loop they would hold dozens of registers)
+      asm volatile("" : "+v"(tid));
       int gone[NC];                                     // a chunk at an end: the last 8 elements, and so many of them dropped
 #pragma unroll
       for (int u = 0; u < NC; ++u) {
@@ -265,39 +278,43 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int NT, bool SINGLE> s
     fetch<T>(v, p, ld, a0, n, r0, rn, R, tid);
     if (DM != PLAIN) fetch<Q>(q, pq, ldq, a0, n, r0, rn, R, tid);
   }
-  // chunk u to LDS; SUMS: the chunk's 8 columns added up (COLS)
-  template <bool SUMS> __device__ __forceinline__ void put(int u, char* lds, float* sums, int tid) {
+  // The way to LDS in pieces of a few instructions, to stand between MFMAs: piece q of PIECES.  SUMS: the 8 columns of the chunks added
+  // up (COLS).
+  static constexpr bool COPY = PL == 1 && DM == PLAIN;
+  static constexpr int PPC = COPY ? 1 : 4 * PL, PIECES = NC * PPC;       // pieces per chunk, in all
+  template <bool SUMS> __device__ __forceinline__ void piece(int q, float (&x)[8], uint32_t (&y)[3][4], char* lds, float* sums, int tid) const {
     constexpr int ROW = SRC == ROWS ? CH : CW;
+    const int u = q / PPC, e = q % PPC / PL, p = q % PL;
+    typedef uint32_t V __attribute__((ext_vector_type(4)));
     const int row = (tid + NT * u) / ROW, c = tid % ROW;
     char* dst = lds + Tl::at(PERM && SRC == ROWS ? perm32(row) : row, c);
-    typedef uint32_t V __attribute__((ext_vector_type(4)));
-    if constexpr (PL == 1 && DM == PLAIN && !SUMS) {    // 16-bit, as it is
+    if (COPY) {
       *(V*)dst = V{v[u].w[0], v[u].w[1], v[u].w[2], v[u].w[3]};
+      if (SUMS) {
+        v[u].floats(x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[i] += x[i];
+      }
       return;
     }
-    float x[8], f[8];
-    v[u].floats(x);
-    if (DM != PLAIN) q[u].floats(f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if (DM == SMOOTH) x[e] *= f[e];
-      if (DM == MASK) x[e] = f[e] > 0.0f ? x[e] : 0.0f;
-      if (SUMS) sums[e] += x[e];
-    }
-#pragma unroll
-    for (int p = 0; p < PL; ++p) {
-      V y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[e] = pack2<L>(x[2 * e], x[2 * e + 1]);
-        if (PL == 3 && p < 2) {                         // the rest for the next bfloat16
-          x[2 * e] -= __builtin_bit_cast(float, y[e] << 16);
-          x[2 * e + 1] -= __builtin_bit_cast(float, y[e] & 0xffff0000u);
-        }
+    if (p == 0) {
+      v[u].pair(e, x[2 * e], x[2 * e + 1]);
+      if (DM != PLAIN) {
+        float f0, f1;
+        q_pair(u, e, f0, f1);
+        if (DM == SMOOTH) { x[2 * e] *= f0; x[2 * e + 1] *= f1; }
+        if (DM == MASK) { x[2 * e] = f0 > 0.0f ? x[2 * e] : 0.0f; x[2 * e + 1] = f1 > 0.0f ? x[2 * e + 1] : 0.0f; }
       }
-      *(V*)(dst + p * Tl::BYTES) = y;
+      if (SUMS) { sums[2 * e] += x[2 * e]; sums[2 * e + 1] += x[2 * e + 1]; }
     }
+    y[p][e] = pack2<L>(x[2 * e], x[2 * e + 1]);
+    if (PL == 3 && p < 2) {                             // the rest for the next bfloat16
+      x[2 * e] -= __builtin_bit_cast(float, y[p][e] << 16);
+      x[2 * e + 1] -= __builtin_bit_cast(float, y[p][e] & 0xffff0000u);
+    }
+    if (e == 3) *(V*)(dst + p * Tl::BYTES) = V{y[p][0], y[p][1], y[p][2], y[p][3]};
   }
+  __device__ __forceinline__ void q_pair(int u, int e, float& a, float& b) const { q[DM != PLAIN ? u : 0].pair(e, a, b); }
 };
 
 // ---- results -----------------------------------------------------------------------------------------------------------------
@@ -339,13 +356,12 @@ template <typename X, int N> __device__ __forceinline__ void store(X* p, const f
   }
 }
 
-// ROWS_ x COLS_ finished values of one wave, wholly inside the output.  MODE: an activation (FORWARD), STORE (as they are) or RAW
+// 32 x COLS_ finished values of one wave, wholly inside the output.  MODE: an activation (FORWARD), STORE (as they are) or RAW
 // (float32 partial sums).
 enum Mode { STORE = 16, RAW = 17 };
-template <typename T, int ROWS_, int COLS_, int EPITCH, int MODE>
+template <typename T, int COLS_, int EPITCH, int MODE>
 __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const float* ep, ll i0, ll j0, int lane) {
   constexpr int C = MODE == RAW || sizeof(T) == 4 ? 4 : 8, LPR = COLS_ / C, RPI = 64 / LPR, UN = 4;
-  static_assert(ROWS_ % (RPI * UN) == 0 || ROWS_ / RPI < UN, "");
   const int col = C * (lane % LPR), row0 = lane / LPR;
   const ll j = j0 + col;
   float b[C];
@@ -355,7 +371,7 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
 #pragma unroll
     for (int e = 0; e < C; ++e) b[e] = (float)((const T*)a.bias)[j + e];
   }
-  constexpr int IT = ROWS_ / RPI, U = IT < UN ? IT : UN;
+  constexpr int IT = 32 / RPI, U = IT < UN ? IT : UN;
 #pragma unroll 1
   for (int it = 0; it < IT; it += U) {
     Chunk<T> r[U];                                     // C elements of the residual (float32: the first half)
@@ -394,24 +410,26 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
   }
 }
 
+template <int N> struct Const { constexpr operator int() const { return N; } };
+
 // ---- the tile kernel ---------------------------------------------------------------------------------------------------------
-template <typename T, int OP, int WI, int WJ, int NI, int NJ> struct Shape {
-  static constexpr int BK = Ty<T>::BK, PL = Ty<T>::PLANES, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
+template <typename T, int OP, int WI, int WJ, int NI, int NJ, int BK> struct Shape {
+  static constexpr int PL = Ty<T>::PLANES, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
   static constexpr int BUF = PL * (BI + BJ) * BK * 2;                               // one step
-  static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * NI * EPITCH * 4;  // the tile on its way out
+  static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
   static constexpr int EXACT = PL == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
   static constexpr int SUMS = OP == BACK_WEIGHT ? NT * 8 * 4 : 0;
   static constexpr int m1 = 2 * BUF > EPI ? 2 * BUF : EPI, m2 = EXACT > SUMS ? EXACT : SUMS, LDS = m1 > m2 ? m1 : m2;
 };
 
-template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, bool SINGLE>
-__global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
-  typedef Shape<T, OP, WI, WJ, NI, NJ> Sh;
+template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK, int OCC, bool SINGLE>
+__global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
+  typedef Shape<T, OP, WI, WJ, NI, NJ, BK> Sh;
   constexpr int SI = OP == BACK_WEIGHT ? COLS : ROWS, SJ = OP == FORWARD ? ROWS : COLS;
-  constexpr int BK = Sh::BK, PL = Sh::PL, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
+  constexpr int PL = Sh::PL, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
   typedef typename Ty<T>::L8 L8;
-  typedef Stage<T, SI, DM, false, BI, NT, SINGLE> StI;
-  typedef Stage<T, SJ, PLAIN, true, BJ, NT, SINGLE> StJ;
+  typedef Stage<T, SI, DM, false, BI, BK, NT, SINGLE> StI;
+  typedef Stage<T, SJ, PLAIN, true, BJ, BK, NT, SINGLE> StJ;
   extern __shared__ __align__(16) char lds[];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -429,58 +447,80 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
   const T* jp = (const T*)a.jp;
   StI si;
   StJ sj;
-  float bs[8] = {};
+  float bs[8] = {}, px[8];
+  uint32_t py[3][4];
   auto fill = [&](ll r) {
     si.load(ip, a.ild, iq, a.iqld, i0, a.I, r, rend, a.R, tid);
     sj.load(jp, a.jld, (const typename StJ::Q*)nullptr, 0, j0, a.J, r, rend, a.R, tid);
   };
-  auto put = [&](int buf) {
+  constexpr int PIECES = StI::PIECES + StJ::PIECES;
+  auto piece = [&](int q, int buf) {
     char* b = lds + buf * Sh::BUF;
-#pragma unroll
-    for (int u = 0; u < StI::NC; ++u) si.template put<OP == BACK_WEIGHT>(u, b, bs, tid);
-#pragma unroll
-    for (int u = 0; u < StJ::NC; ++u) sj.template put<false>(u, b + PL * StI::Tl::BYTES, nullptr, tid);
+    if (q < StI::PIECES) si.template piece<OP == BACK_WEIGHT>(q, px, py, b, bs, tid);
+    else sj.template piece<false>(q - StI::PIECES, px, py, b + PL * StI::Tl::BYTES, nullptr, tid);
   };
 
   const int wi = wave / WJ, wj = wave % WJ;
   f32x16 acc[NI][NJ] = {};
-  auto products = [&](int buf, int kk) {
+  constexpr int READS = (NI + NJ) * PL, MF = NI * NJ * (PL == 3 ? 6 : 1);      // per 16 values of the reduction
+  constexpr int PUT0 = KK > 2 ? KK - 3 : 0, PUTS = KK - 1 - PUT0;              // the sixteens beside which the next step goes to LDS
+  static_assert(KK >= 2, "");
+  struct Operands { L8 i[NI][PL], j[NJ][PL]; };
+  Operands f[2];
+  auto read = [&](Operands& o, int kk, int q, int buf) {
     const char* bi = lds + buf * Sh::BUF;
     const char* bj = bi + PL * StI::Tl::BYTES;
-    L8 fi[NI][PL], fj[NJ][PL];
-#pragma unroll
-    for (int p = 0; p < PL; ++p) {
-#pragma unroll
-      for (int b = 0; b < NI; ++b) fi[b][p] = fragment<L8, SI, BI, BK, false>(bi + p * StI::Tl::BYTES, wi * NI + b, kk, lane);
-#pragma unroll
-      for (int b = 0; b < NJ; ++b) fj[b][p] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b, kk, lane);
-    }
-#pragma unroll
-    for (int sum = PL - 1; sum >= 0; --sum)            // the small products first
-#pragma unroll
-      for (int p = sum; p >= 0; --p)
-#pragma unroll
-        for (int x = 0; x < NI; ++x)
-#pragma unroll
-          for (int y = 0; y < NJ; ++y) acc[x][y] = mfma(fj[y][p], fi[x][sum - p], acc[x][y]);
+    const int p = q / (NI + NJ), b = q % (NI + NJ);
+    if (b < NI) o.i[b % NI][p] = fragment<L8, SI, BI, BK, false>(bi + p * StI::Tl::BYTES, wi * NI + b, kk, lane);
+    else o.j[(b - NI) % NJ][p] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b - NI, kk, lane);
   };
+  auto product = [&](const Operands& o, int q) {       // the small products first
+    constexpr int PI[6] = {2, 0, 1, 0, 1, 0}, PJ[6] = {0, 2, 1, 1, 0, 0};
+    const int t = q / (NI * NJ), x = q % (NI * NJ) / NJ, y = q % NJ;
+    acc[x][y] = mfma(o.j[y][PL == 3 ? PJ[t] : 0], o.i[x][PL == 3 ? PI[t] : 0], acc[x][y]);
+  };
+  // The kk-th 16 values of a step, and between their MFMAs - in this order, a few instructions after each - the reads of the next
+  // sixteen's operands (READ; the last one reads the next step's first, from the other buffer) and pieces of the next step's way to LDS.
+  auto sixteen = [&](auto KK_, auto READ, auto PUT, int buf) {
+    constexpr int kk = KK_, R = READ ? READS : 0;
+    constexpr int P = PUT && kk >= PUT0 && kk < KK - 1 ? PIECES : 0, p0 = P * (kk - PUT0) / PUTS, p1 = P * (kk - PUT0 + 1) / PUTS;
+#pragma unroll
+    for (int q = 0; q < MF; ++q) {
+      product(f[kk & 1], q);
+#pragma unroll
+      for (int e = 2 * R * q / MF; e < 2 * R * (q + 1) / MF; ++e)      // operands in the first half
+        if (e < R) read(f[(kk + 1) & 1], (kk + 1) % KK, e, kk + 1 < KK ? buf : buf ^ 1);
+#pragma unroll
+      for (int e = p0 + (p1 - p0) * q / MF; e < p0 + (p1 - p0) * (q + 1) / MF; ++e) piece(e, buf ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  typedef Const<1> Yes;
+  typedef Const<0> No;
   if (rbeg < rend) {
     fill(rbeg);
-    put(0);
+#pragma unroll
+    for (int q = 0; q < PIECES; ++q) piece(q, 0);
     if (rbeg + BK < rend) fill(rbeg + BK);
     __syncthreads();
-    int buf = 0;
-    for (ll r = rbeg; r + BK < rend; r += BK) {
-      products(buf, 0);
-      put(buf ^ 1);
-      if (r + 2 * BK < rend) fill(r + 2 * BK);
 #pragma unroll
-      for (int kk = 1; kk < KK; ++kk) products(buf, kk);
+    for (int e = 0; e < READS; ++e) read(f[0], 0, e, 0);
+    int buf = 0;
+    // One barrier per step, before its last sixteen: behind it lie the next step's chunks, and nobody reads the buffer that is
+    // written next (its last operands were read before the barrier of the step before).
+    for (ll r = rbeg; r + BK < rend; r += BK) {
+      sixteen(Const<0>(), Yes(), Yes(), buf);
+      if constexpr (KK > 2) sixteen(Const<1>(), Yes(), Yes(), buf);
+      if constexpr (KK > 3) sixteen(Const<2>(), Yes(), Yes(), buf);
+      if (r + 2 * BK < rend) fill(r + 2 * BK);
       __syncthreads();
+      sixteen(Const<KK - 1>(), Yes(), No(), buf);
       buf ^= 1;
     }
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) products(buf, kk);
+    sixteen(Const<0>(), Yes(), No(), buf);
+    if constexpr (KK > 2) sixteen(Const<1>(), Yes(), No(), buf);
+    if constexpr (KK > 3) sixteen(Const<2>(), Yes(), No(), buf);
+    sixteen(Const<KK - 1>(), No(), No(), buf);
   }
 
   if (PL == 3) {
@@ -537,41 +577,49 @@ __global__ __launch_bounds__(64 * WI * WJ, 2) void tile_kernel(const Args a) {
     }
   }
 
-  // the tile leaves through LDS: a lane then finishes 16 bytes of a row, and rows are stored in whole cache lines
-  float* ep = (float*)lds + wave * 32 * NI * EPITCH;
-  __syncthreads();
+  // the tile leaves through LDS, 32 rows of a wave at a time: a lane then finishes 16 bytes of a row, and rows are stored in whole
+  // cache lines
+  float* ep = (float*)lds + wave * 32 * EPITCH;
+  const bool inside = i0 + BI <= a.I && j0 + BJ <= a.J;
+  const ll jw = j0 + wj * NJ * 32;
+#pragma unroll 1
+  for (int x = 0; x < NI; ++x) {
+    __syncthreads();
 #pragma unroll
-  for (int x = 0; x < NI; ++x)
+    for (int v = 0; v < NI; ++v)                       // (registers have no index)
+      if (v == x) {
 #pragma unroll
-    for (int y = 0; y < NJ; ++y)
+        for (int y = 0; y < NJ; ++y)
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *(f32x4*)(ep + (x * 32 + (lane & 31)) * EPITCH + y * 32 + 16 * (lane >> 5) + 4 * q) =
-            f32x4{acc[x][y][4 * q], acc[x][y][4 * q + 1], acc[x][y][4 * q + 2], acc[x][y][4 * q + 3]};
-  __syncthreads();
-  const ll iw = i0 + wi * NI * 32, jw = j0 + wj * NJ * 32;
-  if (i0 + BI <= a.I && j0 + BJ <= a.J) {
-    if (a.part) emit<T, 32 * NI, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, lane);
-    else if (OP != FORWARD) emit<T, 32 * NI, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else if (a.act == NONE) emit<T, 32 * NI, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else if (a.act == RELU) emit<T, 32 * NI, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else if (a.act == SOFTPLUS) emit<T, 32 * NI, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else if (a.act == SIGMOID) emit<T, 32 * NI, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else if (a.act == SILU) emit<T, 32 * NI, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, lane);
-    else emit<T, 32 * NI, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, lane);
-  } else {                                             // a tile at an edge: one element per lane
-    const int rows = a.I - iw < 32 * NI ? (int)(a.I - iw) : 32 * NI, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
-    for (int e = lane; e < rows * cols && cols > 0; e += 64) {
-      const int row = e / cols, col = e % cols;
-      const ll i = iw + row, j = jw + col;
-      float z = ep[row * EPITCH + col], d;
-      if (a.part) {
-        a.part[(s * a.I + i) * a.J + j] = z;
-        continue;
+          for (int q = 0; q < 4; ++q)
+            *(f32x4*)(ep + (lane & 31) * EPITCH + y * 32 + 16 * (lane >> 5) + 4 * q) =
+                f32x4{acc[v][y][4 * q], acc[v][y][4 * q + 1], acc[v][y][4 * q + 2], acc[v][y][4 * q + 3]};
       }
-      if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
-      ((T*)a.out)[i * a.ldo + j] = (T)z;
-      if (OP == FORWARD && a.dact) keep<T>(a, i * a.J + j, d);
+    __syncthreads();
+    const ll iw = i0 + (wi * NI + x) * 32;
+    if (inside) {
+      if (a.part) emit<T, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, lane);
+      else if (OP != FORWARD) emit<T, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else if (a.act == NONE) emit<T, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else if (a.act == RELU) emit<T, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else if (a.act == SOFTPLUS) emit<T, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else if (a.act == SIGMOID) emit<T, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else if (a.act == SILU) emit<T, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, lane);
+      else emit<T, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, lane);
+    } else {                                           // a tile at an edge: one element per lane
+      const int rows = a.I - iw < 32 ? (int)(a.I - iw) : 32, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
+      for (int e = lane; e < rows * cols && cols > 0; e += 64) {
+        const int row = e / cols, col = e % cols;
+        const ll i = iw + row, j = jw + col;
+        float z = ep[row * EPITCH + col], d;
+        if (a.part) {
+          a.part[(s * a.I + i) * a.J + j] = z;
+          continue;
+        }
+        if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
+        ((T*)a.out)[i * a.ldo + j] = (T)z;
+        if (OP == FORWARD && a.dact) keep<T>(a, i * a.J + j, d);
+      }
     }
   }
 
@@ -636,17 +684,25 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
   }
 }
 
-// joins the S partial outputs in order and finishes them like the tile kernel
+// joins the S partial outputs in a fixed order and finishes them like the tile kernel: 64 elements per workgroup, each as 4 sums over
+// every 4th part
 template <typename T, int OP>
 __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
+  __shared__ float buf[4][64];
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
   const ll n = a.I * a.J, extra = OP == BACK_WEIGHT && a.bias_bar ? a.I : 0;
-  const ll e = (ll)blockIdx.x * 256 + threadIdx.x;
-  if (e >= n + extra) return;
-  const float* p = e < n ? a.part + e : a.part_bias + (e - n);
-  const ll step = e < n ? n : a.I;
+  const ll e = (ll)blockIdx.x * 64 + lane;
   float z = 0.0f;
-#pragma unroll 4
-  for (int s = 0; s < a.S; ++s) z += p[s * step];
+  if (e < n + extra) {
+    const float* p = e < n ? a.part + e : a.part_bias + (e - n);
+    const ll step = e < n ? n : a.I;
+#pragma unroll 8
+    for (int s = slice; s < a.S; s += 4) z += p[s * step];
+  }
+  buf[slice][lane] = z;
+  __syncthreads();
+  if (slice != 0 || e >= n + extra) return;
+  z = buf[0][lane] + buf[1][lane] + buf[2][lane] + buf[3][lane];
   if (e >= n) {
     ((T*)a.bias_bar)[e - n] = (T)z;
     return;
@@ -659,37 +715,61 @@ __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
+// Tile variants: rows x columns, workgroups that fit on a CU, and the rate per area at long reductions (8 192 x 4 096 x 4 096 bf16: 64 x 64
+// 480, 128 x 128 880, 256 x 256 1 180 TFLOP/s; 8 192 x 2 048 x 2 048 f32: 64 x 64 130, 256 x 128 212).
+enum Variant { FEW = 0, TINY, SMALL, MIDDLE, LARGE };
+struct Size {
+  int i, j, per_cu;
+  float rate;
+};
+static Size size_of(int dtype, int v) {
+  if (v <= SMALL) return {64, 64, 3, dtype == F32 ? 0.6f : 0.4f};
+  if (v == MIDDLE) return {128, 128, 2, 0.75f};         // 16-bit types
+  return dtype == F32 ? Size{256, 128, 1, 1.0f} : Size{256, 256, 1, 1.0f};
+}
+
 struct Plan {
-  bool few, big, tiny;
-  int S;
+  int variant, S;
   ll TI, TJ, chunk;
 };
 
-// tile edges of the large variant (the small one is 64 x 64)
-static constexpr int big_i(int dtype) { return dtype == F32 ? 256 : 128; }
-static constexpr int big_j(int dtype) { return 128; }
-
-// Which tile and how many splits of the reduction: 256 CUs want at least one workgroup each.
-static Plan plan(int op, int dtype, ll I, ll J, ll R) {
-  const int BK = dtype == F32 ? 32 : 64;
-  auto tiles = [&](int ti, int tj) { return ((I + ti - 1) / ti) * ((J + tj - 1) / tj); };
+// The variant with the least tile area per unit of rate, in whole rounds over 256 CUs, and how many splits of the reduction fill
+// them.  The 256 x 256 tile of the 16-bit types has no registers left for act' beside it.
+static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
+  const int CHUNK = 64;                                 // a multiple of every variant's step
   Plan p = {};
   p.S = 1;
-  p.few = op == FORWARD && I <= 8;
-  if (p.few) return p;
-  p.tiny = R < 8 || I < 8 || J < 8;         // an operand may hold fewer than 8 elements before its end: loaded one by one
-  p.big = !p.tiny && (tiles(big_i(dtype), big_j(dtype)) >= 192 || (I >= 128 && J >= 128 && R >= 8192));
-  const int ti = p.big ? big_i(dtype) : 64, tj = p.big ? big_j(dtype) : 64;
-  const ll n = tiles(ti, tj) < 1 ? 1 : tiles(ti, tj);
-  ll s = n >= 256 ? 1 : 512 / n, most = R / (4 * BK);
-  s = s < most ? s : most;
-  s = s < 1 ? 1 : (s > 512 ? 512 : s);
-  p.chunk = ((R + s - 1) / s + BK - 1) / BK * BK;
-  if (p.chunk < BK) p.chunk = BK;                       // R = 0: the gradient of no rows, one pass over nothing
+  if (op == FORWARD && I <= 8) return p;                // FEW
+  auto tiles = [&](int v) { return ((I + size_of(dtype, v).i - 1) / size_of(dtype, v).i) * ((J + size_of(dtype, v).j - 1) / size_of(dtype, v).j); };
+  const ll longest = R / (dtype == F32 ? 128 : 256) < 1 ? 1 : R / (dtype == F32 ? 128 : 256);      // splits that leave each some work
+  auto splits = [&](int v) {
+    const ll n = tiles(v) < 1 ? 1 : tiles(v), want = 256 * size_of(dtype, v).per_cu;
+    ll s = n * 2 > want ? 1 : want / n;
+    s = s < longest ? s : longest;
+    return s > 512 ? 512 : s;
+  };
+  if (R < 8 || I < 8 || J < 8) p.variant = TINY;        // an operand may hold fewer than 8 elements before its end: loaded one by one
+  else {
+    float best = 0.0f;
+    for (int v = SMALL; v <= LARGE; ++v) {
+      if ((v == MIDDLE && dtype == F32) || (v == LARGE && dtype != F32 && op != FORWARD && act != NONE)) continue;
+      const Size z = size_of(dtype, v);
+      const ll n = tiles(v) * splits(v);
+      const float rounds = n > 2048 ? n / 256.0f : (float)((n + 255) / 256);
+      const float cost = rounds * z.i * z.j / z.rate / splits(v);
+      if (p.variant == FEW || cost < best) {
+        p.variant = v;
+        best = cost;
+      }
+    }
+  }
+  const Size z = size_of(dtype, p.variant);
+  p.chunk = ((R + splits(p.variant) - 1) / splits(p.variant) + CHUNK - 1) / CHUNK * CHUNK;
+  if (p.chunk < CHUNK) p.chunk = CHUNK;                 // R = 0: the gradient of no rows, one pass over nothing
   p.S = (int)((R + p.chunk - 1) / p.chunk);
   if (p.S < 1) p.S = 1;
-  p.TI = (I + ti - 1) / ti;
-  p.TJ = (J + tj - 1) / tj;
+  p.TI = (I + z.i - 1) / z.i;
+  p.TJ = (J + z.j - 1) / z.j;
   return p;
 }
 
@@ -699,20 +779,20 @@ static void shape(int op, ll m, ll n, ll k, ll& I, ll& J, ll& R) {
   R = op == FORWARD ? k : (op == BACK_DATA ? n : m);
 }
 
-long long workspace_bytes(int op, int dtype, long long m, long long n, long long k) {
+long long workspace_bytes(int op, int dtype, int act, long long m, long long n, long long k) {
   ll I, J, R;
   shape(op, m, n, k, I, J, R);
-  const Plan p = plan(op, dtype, I, J, R);
+  const Plan p = plan(op, dtype, act, I, J, R);
   return p.S == 1 ? 0 : 4 * (ll)p.S * (I * J + (op == BACK_WEIGHT ? I : 0));
 }
 
 // more than 64 KB of LDS has to be asked for, once per kernel and device (idempotent: no lock)
-template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, bool SINGLE = false> static int start(const Args& a, unsigned grid, hipStream_t st) {
-  typedef Shape<T, OP, WI, WJ, NI, NJ> Sh;
+template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK, int OCC, bool SINGLE = false> static int start(const Args& a, unsigned grid, hipStream_t st) {
+  typedef Shape<T, OP, WI, WJ, NI, NJ, BK> Sh;
   static bool ready[64];
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -2;
-  auto* kernel = tile_kernel<T, OP, DM, WI, WJ, NI, NJ, SINGLE>;
+  auto* kernel = tile_kernel<T, OP, DM, WI, WJ, NI, NJ, BK, OCC, SINGLE>;
   if (!ready[dev]) {
     if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, Sh::LDS) != hipSuccess) return -2;
     ready[dev] = true;
@@ -721,19 +801,25 @@ template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, bool SINGL
   return 0;
 }
 
-template <typename T, int OP, int DM> static int start_tile(const Args& a, bool big, bool tiny, unsigned grid, hipStream_t st) {
-  if (tiny) return start<T, OP, DM, 2, 2, 1, 1, true>(a, grid, st);
-  if (!big) return start<T, OP, DM, 2, 2, 1, 1>(a, grid, st);
-  if constexpr (sizeof(T) == 4) return start<T, OP, DM, 4, 2, 2, 2>(a, grid, st);
-  else return start<T, OP, DM, 2, 2, 2, 2>(a, grid, st);
+template <typename T, int OP, int DM> static int start_tile(const Args& a, int variant, unsigned grid, hipStream_t st) {
+  if (variant == TINY) return start<T, OP, DM, 2, 2, 1, 1, 32, 2, true>(a, grid, st);
+  if constexpr (sizeof(T) == 4) {
+    if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 32, 2>(a, grid, st);
+    return start<T, OP, DM, 4, 2, 2, 2, 32, 2>(a, grid, st);
+  } else {
+    if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 64, 2>(a, grid, st);
+    if constexpr (DM == PLAIN)
+      if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, 64, 2>(a, grid, st);
+    return start<T, OP, DM, 2, 2, 2, 2, 64, 2>(a, grid, st);
+  }
 }
 
 template <typename T, int OP>
 static int run(const Call& c, hipStream_t st) {
   Args a = {};
   shape(OP, c.m, c.n, c.k, a.I, a.J, a.R);
-  const Plan p = plan(OP, c.dtype, a.I, a.J, a.R);
-  const ll need = workspace_bytes(OP, c.dtype, c.m, c.n, c.k);
+  const Plan p = plan(OP, c.dtype, c.act, a.I, a.J, a.R);
+  const ll need = workspace_bytes(OP, c.dtype, c.act, c.m, c.n, c.k);
   if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
   a.ip = OP == FORWARD ? c.x : c.ybar;
   a.ild = OP == FORWARD ? c.ldx : c.ldyb;
@@ -759,7 +845,7 @@ static int run(const Call& c, hipStream_t st) {
     a.part_bias = a.part + (ll)p.S * a.I * a.J;
   }
   if constexpr (OP == FORWARD) {
-    if (p.few) {
+    if (p.variant == FEW) {
       const dim3 grid((unsigned)((a.J + 3) / 4));
       switch (a.I) {
         case 1: few_kernel<T, 1><<<grid, 256, 0, st>>>(a); break;
@@ -776,13 +862,13 @@ static int run(const Call& c, hipStream_t st) {
   }
   const unsigned grid = (unsigned)(p.TI * p.TJ * p.S);
   int rc;
-  if constexpr (OP == FORWARD) rc = start_tile<T, OP, PLAIN>(a, p.big, p.tiny, grid, st);
-  else rc = c.act == NONE ? start_tile<T, OP, PLAIN>(a, p.big, p.tiny, grid, st) : (c.act == RELU ? start_tile<T, OP, MASK>(a, p.big, p.tiny, grid, st)
-                                                                                          : start_tile<T, OP, SMOOTH>(a, p.big, p.tiny, grid, st));
+  if constexpr (OP == FORWARD) rc = start_tile<T, OP, PLAIN>(a, p.variant, grid, st);
+  else rc = c.act == NONE ? start_tile<T, OP, PLAIN>(a, p.variant, grid, st) : (c.act == RELU ? start_tile<T, OP, MASK>(a, p.variant, grid, st)
+                                                                                          : start_tile<T, OP, SMOOTH>(a, p.variant, grid, st));
   if (rc) return rc;
   if (p.S > 1) {
     const ll n = a.I * a.J + (a.bias_bar ? a.I : 0);
-    reduce_kernel<T, OP><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(a);
+    reduce_kernel<T, OP><<<dim3((unsigned)((n + 63) / 64)), 256, 0, st>>>(a);
   }
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }

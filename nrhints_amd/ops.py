@@ -393,7 +393,7 @@ def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
     dact = None
     if want_dact and code != 0 and not (code == 1 and residual is None):
         dact = x.new_empty(shape, dtype=x.dtype if code == 1 else _DACT[x.dtype])
-    ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 0, dtype, m, n, k)
+    ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 0, dtype, code, m, n, k)
     with _Here(x.device) as stream:
         rc = _lib.load().nrh_linear_forward(dtype, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _vp(b1), _vp(r2), ldr, code, beta, m, n, k,
                                             y.data_ptr(), n, _vp(dact), _vp(ws), nbytes, stream)
@@ -439,11 +439,11 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
     b_bar = x.new_empty((n,)) if want_bias else None
     with _Here(x.device) as stream:
         if want_x:
-            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 1, dtype, m, n, k)
+            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 1, dtype, code, m, n, k)
             _lib.check(lib.nrh_linear_backward_data(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, w2.data_ptr(), ldw, m, n, k,
                                                     x_bar.data_ptr(), k, _vp(ws), nbytes, stream), "nrh_linear_backward_data")
         if w_bar is not None:
-            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 2, dtype, m, n, k)
+            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 2, dtype, code, m, n, k)
             _lib.check(lib.nrh_linear_backward_weight(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, x2.data_ptr(), ldx, m, n, k,
                                                       w_bar.data_ptr(), k, _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
     return x_bar, (w_bar if want_weight else None), b_bar

@@ -92,7 +92,7 @@ def check_linear(x, w, b, r, yb, act, beta, train=True):
 
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 7, 3), (5, 1024, 513), (16, 40, 8), (31, 256, 1), (33, 33, 33), (64, 64, 64), (65, 129, 63), (127, 84, 256),
-         (128, 128, 128), (129, 340, 256), (300, 361, 255), (1000, 63, 129), (4099, 256, 3), (8192, 256, 256), (20000, 39, 217)]
+         (128, 128, 128), (129, 340, 256), (300, 361, 255), (1000, 63, 129), (4099, 256, 3), (8192, 256, 256), (20000, 39, 217), (16500, 1000, 1030), (3000, 2050, 2000)]
 
 
 @pytest.mark.parametrize("dtype", DT, ids=IDS)
@@ -238,7 +238,7 @@ def test_linear_writes_only_its_own_columns(dtype):
     for ldx in (k, k + 3):
         bx = torch.full((m, ldx), 7.0, dtype=dtype, device="cuda")
         bw = torch.full((n, ldx), 7.0, dtype=dtype, device="cuda")
-        ws = [torch.empty(max(1, lib.nrh_linear_workspace_bytes(op, code, m, n, k)), dtype=torch.uint8, device="cuda") for op in (1, 2)]
+        ws = [torch.empty(max(1, lib.nrh_linear_workspace_bytes(op, code, 0, m, n, k)), dtype=torch.uint8, device="cuda") for op in (1, 2)]
         assert lib.nrh_linear_backward_data(code, P(yb), n, None, 0, 0, P(w), k, m, n, k, P(bx), ldx, P(ws[0]), ws[0].numel(), _lib.stream_handle()) == 0
         assert lib.nrh_linear_backward_weight(code, P(yb), n, None, 0, 0, P(x), k, m, n, k, P(bw), ldx, None, P(ws[1]), ws[1].numel(), _lib.stream_handle()) == 0
         xb, wb, _ = ops.linear_backward(yb, x, w, None)

@@ -27,8 +27,8 @@ def test_c_entries_refuse_bad_arguments():
     assert fwd(m=0, x=None, y=None) == 0                   # no rows: nothing to do
     for bad in (dict(act=1), dict(d=p, ldd=4), dict(act=4, d=p, ldd=3), dict(ldo=7), dict(ldg=3), dict(g=None), dict(o=None), dict(m=1 << 31)):
         assert data(**bad) == -1, bad
-    assert lib.nrh_linear_workspace_bytes(3, 0, 1, 1, 1) == -1 and lib.nrh_linear_workspace_bytes(0, 0, 1, 0, 1) == -1
-    need = lib.nrh_linear_workspace_bytes(2, 0, 100000, 256, 256)
+    assert lib.nrh_linear_workspace_bytes(3, 0, 0, 1, 1, 1) == -1 and lib.nrh_linear_workspace_bytes(0, 0, 0, 1, 0, 1) == -1
+    need = lib.nrh_linear_workspace_bytes(2, 0, 0, 100000, 256, 256)
     assert need > 0
     assert lib.nrh_linear_backward_weight(0, p, 256, None, 0, 0, p, 256, 100000, 256, 256, p, 256, None, None, 0, None) == -3
     assert lib.nrh_linear_backward_weight(0, p, 256, None, 0, 0, p, 256, 100000, 256, 256, p, 256, None, p, need - 1, None) == -3
@@ -51,9 +51,9 @@ def test_workspace_sizes_cover_every_shape():
     for m in (0, 1, 17, 300, 4096, 163840, 655360, 1 << 30):
         for n in (1, 3, 64, 129, 256, 1024):
             for k in (1, 39, 84, 256, 361, 4096):
-                for dtype in (0, 1, 2):
+                for dtype, act in ((0, 0), (1, 0), (2, 0), (2, 1), (1, 4)):
                     for op, out in ((0, m * n), (1, m * k), (2, n * k + n)):
-                        b = lib.nrh_linear_workspace_bytes(op, dtype, m, n, k)
+                        b = lib.nrh_linear_workspace_bytes(op, dtype, act, m, n, k)
                         assert b >= 0 and (b == 0 or (b % (4 * out) == 0 and b // (4 * out) <= 512 and b < 1 << 31)), (op, m, n, k, b)
 
 
