@@ -8,8 +8,8 @@
 //             tile of 1 024 tokens, ranked scatter; the scan between them is part of the scatter up to 64 tiles).
 //             sum: a group of lanes - one lane per 16 bytes of a row - walks 32 sorted tokens.  A run that begins and ends inside is
 //             written to the table; the first and the last run of a group may go on in its neighbours and are handed, as float32
-//             rows with their keys, to the next level, which does the same, until one group is left.  A
-//             row named by every token and a table named once per row cost the same.  Rows that no token names are found by bisection
+//             rows with their keys, to the next level, which does the same with 16 entries per group, until one group is left.  A row
+//             named by every token and a table named once per row cost the same.  Rows that no token names are found by bisection
 //             in the sorted keys and cleared beside the first level: every row is written once.
 // Both directions are bound by HBM at large sizes (the tokens' rows are read once, the table's gradient is written once), by launches
 // at small ones.
@@ -22,7 +22,7 @@ namespace nrhemb {
 typedef long long ll;
 typedef unsigned long long ull;
 constexpr unsigned NONE = 0xffffffffu;
-constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 32, LOW = 255, LOW_TOKENS = 512;
+constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 16, LOW = 255, LOW_TOKENS = 512;
 
 template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
 template <typename T> struct Vec<T, 1> { typedef T type; };

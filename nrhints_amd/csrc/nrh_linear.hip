@@ -234,7 +234,8 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool S
   // addresses of one uniform base per chunk plus one 32-bit lane offset; at the edges every chunk is checked.
   template <typename X> static __device__ __forceinline__ void fetch(Chunk<X>* c, const X* p, ll ld, ll a0, ll n, ll r0, ll rn, ll R, int tid) {
     constexpr int ROW = SRC == ROWS ? CH : CW, STEP = NT / ROW;
-    if (a0 + BA <= n && r0 + BK <= rn && ld < (1 << 22)) {
+    const bool axis = a0 + BA <= n || (SRC == COLS && (R - r0 - BK) * ld + n >= a0 + BA);      // (COLS: rows enough behind the step)
+    if (axis && r0 + BK <= rn && ld < (1 << 22)) {
       const X* base = p + (SRC == ROWS ? a0 * ld + r0 : r0 * ld + a0);
       const unsigned lane = (unsigned)(tid / ROW) * (unsigned)ld + 8 * (tid % ROW);
 #pragma unroll
