@@ -7,7 +7,8 @@ network, and all their adjoints - stays in the HIP kernels (``nrh_sample_primary
 ``NrhNet.bg_alpha``, ``nrh_alpha_blend_*``).  The background network itself - an 8 x 256 ReLU MLP with a skip connection, a density
 head and a 128-wide view branch - is the kernel pair of csrc/nrh_outside.hip (``nrh_outside_forward`` / ``nrh_outside_backward``, the
 transposed register chain of the other per-point networks, both precisions) and its weight gradients are jobs of ``nrh_dw_gemm``;
-there is no library GEMM and no autograd inside the network.  What stays in torch is elementwise work on [N,160] arrays: the sample
+there is no library GEMM and no autograd inside the network.  At another shape (wider, other depths, skips or encodings) the network is
+composed of ``layers.linear`` calls instead (float32, csrc/nrh_linear.hip), everything around it unchanged.  What stays in torch is elementwise work on [N,160] arrays: the sample
 positions, alpha = 1 - exp(-softplus(density) dist), the 32-sample tail composite, and the chain rule through the two positional
 encodings for the ray gradients.
 """
@@ -21,8 +22,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from . import _lib, dw
-from .autograd_core import _freqs
+from . import _lib, dw, layers
+from .autograd_core import _enc, _freqs
 from .packing import pack_stage, pack_stage_h3
 
 N_OUTSIDE = 32
@@ -46,15 +47,18 @@ class _Affine(nn.Module):
 class OutsideNeRF(nn.Module):
     """The reference's ``NeRF`` (fields/nerf_density_field.py:30-89) with its state-dict names: pts_linears.0..7, views_linears.0,
     feature_linear, alpha_linear, rgb_linear (constructed in the reference's order, so the init RNG stream of a model built with
-    the background matches too).  ``forward`` runs csrc/nrh_outside.hip (GPU tensors only)."""
+    the background matches too).  ``forward`` (GPU tensors only) runs csrc/nrh_outside.hip where the shape is the compiled one - 8 x 256,
+    encodings 10 + 4, skips [4] - and a chain of ``layers.linear`` at any other."""
 
-    precision = "f16x3"      # set by the renderer that owns the module
+    precision = "f16x3"      # set by the renderer that owns the module (the compiled shape; the other shapes are float32)
 
     def __init__(self, d_in: int = 4, d_in_view: int = 6, d_hidden: int = 256, n_layers: int = 8, multi_res: int = 10,
                  multi_res_view: int = 4, skips=(4,)):
         super().__init__()
-        if (d_in, d_in_view, d_hidden, n_layers, multi_res, multi_res_view, tuple(skips)) != (4, 6, 256, 8, 10, 4, (4,)):
-            raise ValueError("the outside-NeRF kernels are built for the default 8 x 256 / multires 10 + 4 / skips = [4] network")
+        if d_in < 1 or d_in_view != 6 or d_hidden < 2 or d_hidden % 2 or n_layers < 1 or multi_res < 0 or multi_res_view < 0 or \
+                any(not 0 <= i < n_layers - 1 for i in skips):
+            raise ValueError("OutsideNeRF: view and light inputs (d_in_view = 6), an even d_hidden, skips among the layers before the last")
+        self.compiled = (d_in, d_hidden, n_layers, multi_res, multi_res_view, tuple(skips)) == (4, 256, 8, 10, 4, (4,))
         self.multi_res, self.multi_res_view, self.skips = multi_res, multi_res_view, tuple(skips)
         ch, ch_view = d_in * (2 * multi_res + 1), d_in_view * (2 * multi_res_view + 1)
         self.pts_linears = nn.ModuleList([_Affine(ch, d_hidden)] + [
@@ -71,7 +75,28 @@ class OutsideNeRF(nn.Module):
 
     def forward(self, pts4: torch.Tensor, views: torch.Tensor, pls: torch.Tensor, pts_per_ray: int = 1) -> Tuple[torch.Tensor, torch.Tensor]:
         """pts4 [P,4]; views, pls [P / pts_per_ray, 3] -> (density [P,1], rgb before the sigmoid [P,3])  (:66-89)."""
-        return OutsideNetHip.apply(pts4, views, pls, _lib.PRECISIONS[self.precision], int(pts_per_ray), *self.ordered_parameters())
+        if self.compiled:
+            return OutsideNetHip.apply(pts4, views, pls, _lib.PRECISIONS[self.precision], int(pts_per_ray), *self.ordered_parameters())
+        return self._layered(pts4, views, pls, int(pts_per_ray))
+
+    def _layered(self, pts4: torch.Tensor, views: torch.Tensor, pls: torch.Tensor, pts_per_ray: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The same network layer by layer on ``layers.linear`` (:66-89): autograd joins the layers and the two encodings, and each
+        layer's product with its gradients is csrc/nrh_linear.hip."""
+        if not pts4.is_cuda:
+            raise RuntimeError("the outside-NeRF network runs on the GPU only (csrc/nrh_linear.hip)")
+        if views.shape[0] * pts_per_ray != pts4.shape[0] or pls.shape != views.shape:
+            raise ValueError("views / pls must hold one row per group of pts_per_ray points")
+        step = lambda m, x, act="none": layers.linear(x, m.weight, m.bias, activation=act)
+        x = _enc(pts4.to(torch.float32), self.multi_res)
+        v = _enc(torch.cat([views, pls], dim=-1).to(torch.float32), self.multi_res_view)
+        h = x
+        for i, m in enumerate(self.pts_linears):
+            h = step(m, h, "relu")
+            if i in self.skips:
+                h = torch.cat([x, h], dim=-1)
+        rays = v[:, None, :].expand(-1, pts_per_ray, -1).reshape(pts4.shape[0], v.shape[1])
+        hv = step(self.views_linears[0], torch.cat([step(self.feature_linear, h), rays], dim=-1), "relu")
+        return step(self.alpha_linear, h), step(self.rgb_linear, hv)
 
 
 def pack_outside(params: List[torch.Tensor], precision: int, transposed: bool):

@@ -9,7 +9,8 @@ On the GPU a bundle is one HIP launch (``nrh_generate_rays_indexed``): the per-V
 the adjustment, [V,3,4] - are composed with a handful of tiny torch ops (differentiable, V ~ 100), the per-RAY work
 (pose composition, pixel -> direction, normalisation, light offset, near/far) runs in the kernel, and its adjoint kernel
 scatters the ray gradients the HIP training path provides (origins / directions / pl_positions / nears / fars) back into
-d/d(delta) with atomics.  CPU tensors take the same formulas as torch ops (the form the CPU parity test checks against the
+d/d(delta) with atomics - or, with ``RayGenerator(deterministic=True)``, through ``layers.embedding``: the deltas are looked up per ray
+and their gradients summed by sorted view index, in a fixed order (the same bits on every run).  CPU tensors take the same formulas as torch ops (the form the CPU parity test checks against the
 reference's fixture).  Whole evaluation views without refinement use ``pipeline.generate_rays``.
 """
 from __future__ import annotations
@@ -128,8 +129,11 @@ class RayGenerator(nn.Module):
     """``forward(RawPixelBundle) -> RayBundle`` (camera/ray_generator.py:75-150)."""
 
     def __init__(self, camera: CameraModel, num_cameras: int, config: RayGeneratorConfig = None, zn: float = 0.1,
-                 zf: float = 10.0):
+                 zf: float = 10.0, deterministic: bool = False):
+        """``deterministic`` (GPU): gradients of the per-view deltas repeat bit for bit (several rays of a batch share a view; their
+        contributions are otherwise added in the order the hardware finishes them).  The rays are the same bits either way."""
         super().__init__()
+        self.deterministic = bool(deterministic)
         self.camera = camera
         self.config = cfg = RayGeneratorConfig() if config is None else config
         self.zn, self.zf = float(getattr(camera, "zn", zn)), float(getattr(camera, "zf", zf))
@@ -206,11 +210,27 @@ class RayGenerator(nn.Module):
             self.__dict__["_idx_validated"] = True
         cc = lambda t: None if t is None else t.contiguous().float()
         poses = f32(pb.poses)
+        if self.deterministic and idx is not None and (delta is not None or pl_delta is not None):
+            delta, pl_delta, idx = self._rows_per_ray(delta, pl_delta, idx)
         o, d, p, near, far = _RaysIndexedHip.apply(cc(delta), cc(pl_delta), idx, f32(pb.h_indices).reshape(-1),
                                                    f32(pb.w_indices).reshape(-1), poses, f32(pb.pls),
                                                    (float(cam.cx), float(cam.cy), float(cam.fx), float(cam.fy),
                                                     bool(cfg.override_near_far_from_sphere), self.zn, self.zf))
         return RayBundle(origins=o, directions=d, pl_positions=p, nears=near, fars=far)
+
+    @staticmethod
+    def _rows_per_ray(delta, pl_delta, idx):
+        """Every ray's own row of the delta tables, and the ray's own number as its index: the adjoint kernel then adds exactly one
+        contribution to each row, and ``layers.embedding``'s gradient sums the rows of a view in their order.  A view index outside the
+        tables stays "no refinement" (index -1; its row is not read)."""
+        from . import layers
+        rows = int((delta if delta is not None else pl_delta).shape[0])
+        own = torch.where((idx >= 0) & (idx < rows), torch.arange(idx.numel(), device=idx.device), -1)
+        if delta is not None:
+            delta = layers.embedding(delta.contiguous().float().reshape(rows, 12), idx).reshape(-1, 3, 4)
+        if pl_delta is not None:
+            pl_delta = layers.embedding(pl_delta.contiguous().float(), idx)
+        return delta, pl_delta, own
 
     def forward(self, pixel_bundle: RawPixelBundle) -> RayBundle:
         cam, cfg = self.camera, self.config

@@ -76,3 +76,24 @@ def test_modules_initialise_like_torch():
     for bad in (lambda: layers.Linear(0, 3), lambda: layers.Linear(3, 3, activation="tanh"), lambda: layers.Embedding(0, 3)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_background_network_shapes():
+    """outside_nerf beyond the compiled shape is accepted (layers.linear), with the reference's layer sizes; what no layer chain can run
+    and networks narrower than the compiled one are refused."""
+    import nrhints_amd as na
+    on = na.NeuSRendererConfig(use_outside_nerf=True)
+    wide = na.NeuSModelConfig(renderer=on, outside_nerf=na.NeRFConfig(d_hidden=512, n_layers=6, multi_res=8, multi_res_view=3, skips=[2, 4]))
+    assert na.unsupported_reason(wide) is None
+    m = na.NeuSHintRenderer(wide).outside_nerf
+    assert not m.compiled and na.NeuSHintRenderer(na.NeuSModelConfig(renderer=on)).outside_nerf.compiled
+    ch, cv = 4 * 17, 6 * 7
+    assert [tuple(l.weight.shape) for l in m.pts_linears] == [(512, ch), (512, 512), (512, 512), (512, 512 + ch), (512, 512), (512, 512 + ch)]
+    assert m.views_linears[0].weight.shape == (256, 512 + cv) and m.alpha_linear.weight.shape == (1, 512) and m.rgb_linear.weight.shape == (3, 256)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        m(torch.zeros(4, 4), torch.zeros(1, 3), torch.zeros(1, 3), pts_per_ray=4)
+    for bad in (dict(d_hidden=300, n_layers=4, skips=[3]), dict(d_hidden=257), dict(d_hidden=255), dict(d_hidden=64), dict(skips=[7]), dict(skips=[-1]), dict(multi_res=0),
+                dict(n_layers=1, skips=[])):
+        assert na.unsupported_reason(na.NeuSModelConfig(renderer=on, outside_nerf=na.NeRFConfig(**bad))), bad
+        # (off by default: a network that is not built is not looked at)
+        assert na.unsupported_reason(na.NeuSModelConfig(outside_nerf=na.NeRFConfig(**bad))) is None
