@@ -279,7 +279,7 @@ def timed_render(model, rb, bg, steps, warmup, dist, dev, sharded, n_total=None)
     _lib.check(lib.nrh_kernel_timing_select(-1), "timing_select")
     if dist is not None:
         t = torch.tensor([dt], dtype=torch.float64, device=dev)
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        parallel.all_reduce(t, dist.ReduceOp.MAX)
         dt = float(t.item())
     return dt, out, k_ms.value, max(1, k_n.value), float(stats.get("host_s", 0.0))
 
@@ -445,8 +445,9 @@ def train_leg(dev, rank, world, dist, batch=1024, steps=30, warm=3, global_batch
         block_s.append(time.perf_counter() - t0)
     dt = sorted(block_s)[len(block_s) // 2]
     if dist is not None:
+        from nrhints_amd import parallel
         t = torch.tensor([dt], dtype=torch.float64, device=dev)
-        dist.all_reduce(t, op=dist.ReduceOp.MAX)
+        parallel.all_reduce(t, dist.ReduceOp.MAX)
         dt = float(t.item())
     graphed.release()
     losses = [float(x) for x in losses]
@@ -522,7 +523,7 @@ def main():
     if world > 1:
         import torch.distributed as dist
         # RCCL on ROCm ("nccl"): barrier, max-over-ranks, pixel all-gather, gradient all-reduce.  RCCL refuses two ranks on one device,
-        # hence gloo (which stages device tensors through the host) for the one-GPU rehearsal - its numbers are not a benchmark
+        # hence gloo (on host copies, parallel._staged) for the one-GPU rehearsal - its numbers are not a benchmark
         dist.init_process_group(backend="gloo" if SHARE_GPU else "nccl")
     # what the process group actually is (reported in the line, so that a multi-GPU run certifies itself): backend, world size as
     # the collective library sees it, and every rank's device
@@ -533,8 +534,9 @@ def main():
             mine = f"rank {rank}: cuda:{local_rank} {torch.cuda.get_device_name(local_rank)} pci {getattr(props, 'pci_bus_id', '?')} pid {os.getpid()}"
             gathered = [None] * world
             dist.all_gather_object(gathered, mine)
+            from nrhints_amd import parallel
             probe = torch.ones(1, device=dev)
-            dist.all_reduce(probe)                       # a device collective through the backend: sum of ones = ranks that took part
+            parallel.all_reduce(probe)                       # a device collective through the backend: sum of ones = ranks that took part
             comm = {"backend": dist.get_backend(), "world_size": dist.get_world_size(), "all_reduce_of_ones": float(probe.item()),
                     "devices": gathered}
         except Exception as e:  # noqa: BLE001 - a report, never a reason for the benchmark to stop

@@ -532,7 +532,8 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
       for (int y = 0; y < NJ; ++y)
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          bad |= !(fabsf(acc[x][y][e]) < __builtin_huge_valf()) && j0 + (wj * NJ + y) * 32 + 16 * (lane >> 5) + e < a.J;
+          bad |= !(fabsf(acc[x][y][e]) < __builtin_huge_valf()) && j0 + (wj * NJ + y) * 32 + 16 * (lane >> 5) + e < a.J &&
+                 i0 + (wi * NI + x) * 32 + (lane & 31) < a.I;
     if (__syncthreads_or(bad)) {                       // float32 products: rows of BK + 1 floats, two values of the reduction per MFMA
       float* fl = (float*)lds;
 #pragma unroll

@@ -4,7 +4,8 @@ csrc/nrh_embedding.hip).
 The networks of the renderer run on kernels whose shape is compiled in; these are the building blocks for networks that have another
 one (the background network at other widths and depths, outside.OutsideNeRF) and for tables looked up per ray (RayGenerator's
 per-view deltas).  GPU tensors only, float32 / float16 / bfloat16, one derivative (a second one raises).  Gradients are summed in a
-fixed order: the same bits on every run.
+fixed order: the same bits on every run.  Forward and backward may be captured into a graph; a capture is refused while an eager graph
+of the same parameters is alive.
 """
 from __future__ import annotations
 
@@ -14,8 +15,27 @@ from typing import Optional
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import get_gradient_edge
 
 from . import ops
+
+
+_EAGER = "nrhints_amd.layers: recorded outside a capture"
+
+
+def _same_side_of_capture(*tensors) -> None:
+    """A parameter's gradient is accumulated on the stream its graph was first recorded on.  If an eager graph of the parameter is still
+    alive, a backward pass captured now would accumulate on the eager stream and end the process: refuse it here, while an exception
+    still can."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    for t in tensors:
+        if t is not None and t.requires_grad and t.is_leaf:
+            meta = get_gradient_edge(t).node.metadata
+            if not capturing:
+                meta[_EAGER] = True
+            elif _EAGER in meta:
+                raise RuntimeError("a graph recorded outside this capture still holds one of these parameters: delete its outputs "
+                                   "(or detach them) before capturing")
 
 
 class LinearHip(torch.autograd.Function):
@@ -25,6 +45,7 @@ class LinearHip(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation: str, beta: float):
         if not any(ctx.needs_input_grad[:3]):
             return ops.linear(x, weight, bias, residual, activation, beta)
+        _same_side_of_capture(x, weight, bias, residual)
         y, dact = ops.linear_train_forward(x, weight, bias, residual, activation, beta)
         ctx.save_for_backward(x, weight, dact)      # relu without residual: dact is y, an output (saved as such, no copy)
         ctx.activation = activation
@@ -46,6 +67,8 @@ class EmbeddingHip(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, index, scale: float):
+        if ctx.needs_input_grad[0]:
+            _same_side_of_capture(table)
         ctx.save_for_backward(index)
         ctx.rows, ctx.scale = table.shape[0], float(scale)
         return ops.embedding(table, index, scale)

@@ -35,6 +35,33 @@ def views_of_rank(n_views: int, rank: int, world: int, skip: int = 1) -> List[in
     return list(range(rank * skip, n_views, skip * world))
 
 
+def _staged(collective, tensors, group) -> None:
+    """Run ``collective`` on ``tensors``, or - device tensors over gloo (rehearsals of several ranks on one GPU) - on host copies: gloo is
+    handed CPU tensors only, copied synchronously, since its own staging of device tensors has hung with several ranks on one GPU."""
+    if dist.get_backend(group) != "gloo" or not any(t.is_cuda for t in tensors):
+        collective(*tensors)
+        return
+    host = [t.cpu() for t in tensors]
+    collective(*host)
+    for t, h in zip(tensors, host):
+        t.copy_(h)
+
+
+def all_reduce(t: torch.Tensor, op=dist.ReduceOp.SUM, group: Optional[dist.ProcessGroup] = None) -> None:
+    """``dist.all_reduce`` in place on any backend (host copies over gloo)."""
+    _staged(lambda x: dist.all_reduce(x, op=op, group=group), [t], group)
+
+
+def broadcast(t: torch.Tensor, src: int = 0, group: Optional[dist.ProcessGroup] = None) -> None:
+    """``dist.broadcast`` in place on any backend (host copies over gloo)."""
+    _staged(lambda x: dist.broadcast(x, src=src, group=group), [t], group)
+
+
+def all_gather_into(recv: torch.Tensor, send: torch.Tensor, group: Optional[dist.ProcessGroup] = None) -> None:
+    """``dist.all_gather_into_tensor`` on any backend (host copies over gloo)."""
+    _staged(lambda r, x: dist.all_gather_into_tensor(r, x, group=group), [recv, send], group)
+
+
 # (device, dtype, rows, columns, world) -> (send [cap, C], recv [world * cap, C]): allocated once, reused by every frame
 _GATHER_BUFFERS: Dict[tuple, Tuple[torch.Tensor, torch.Tensor]] = {}
 
@@ -79,7 +106,7 @@ def render_slab(render_fn: Callable[[RayBundle], "object"], my_rays: RayBundle, 
     for t, w in zip(parts, widths):
         send[: hi - lo, c: c + w].copy_(t.reshape(hi - lo, w))
         c += w
-    dist.all_gather_into_tensor(recv, send, group=group)
+    all_gather_into(recv, send, group)
     if n_total % world == 0:
         frame = recv                                   # slabs are contiguous and unpadded: the buffer IS the frame
     else:

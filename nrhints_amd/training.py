@@ -19,6 +19,8 @@ import torch
 import torch.distributed as dist
 from torch import nn
 
+from . import parallel
+
 
 def train_loss_dict(out, rgb_gt: torch.Tensor, igr_weight: float = 0.1) -> Dict[str, torch.Tensor]:
     """``out``: RenderOutput of ``forward(..., is_training=True)``; returns loss / rgb_loss / eikonal_loss / s_val / psnr."""
@@ -79,7 +81,7 @@ class FlatGradAllReduce:
             return
         with torch.no_grad():
             flat = torch.cat([p.detach().reshape(-1) for p in self.params])
-            dist.broadcast(flat, src=src, group=self.group)
+            parallel.broadcast(flat, src, self.group)
             off = 0
             for p in self.params:
                 p.copy_(flat[off: off + p.numel()].view_as(p))
@@ -121,7 +123,7 @@ class FlatGradAllReduce:
         """The one collective of a step (RCCL ring over xGMI; 3.3 MB of fp32 gradients for the default networks).  RCCL averages
         in the collective (ReduceOp.AVG); gloo (CPU tests, one-GPU rehearsal) sums and unpack() divides."""
         self._avg = dist.get_backend(self.group) == "nccl"
-        dist.all_reduce(self._flat, op=dist.ReduceOp.AVG if self._avg else dist.ReduceOp.SUM, group=self.group)
+        parallel.all_reduce(self._flat, dist.ReduceOp.AVG if self._avg else dist.ReduceOp.SUM, self.group)
 
     def unpack(self) -> None:
         """Flat buffer / world size -> gradients (graph-capturable; in place - at most the division - when pack() found the

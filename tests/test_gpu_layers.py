@@ -467,3 +467,34 @@ def test_a_captured_backward_pass():
         gr.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(eager, grads))
+
+
+def test_a_capture_beside_a_live_eager_graph_is_refused():
+    """Parameters whose eager graph still lives would accumulate their gradients on the eager stream from inside a capture: refused with an
+    exception; once the graph is gone the same capture works."""
+    torch.manual_seed(2)
+    net = Net().cuda()
+    x, view, seed = torch.randn(64, 39, device="cuda"), torch.randint(0, 20, (64,), device="cuda"), torch.randn(64, 3, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = torch.autograd.grad(net(x, view), list(net.parameters()), seed)      # warm-up, its graph ends here
+    torch.cuda.current_stream().wait_stream(side)
+    alive = net(x, view)
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            net(x, view)
+    torch.cuda.synchronize()
+    del alive
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        y = net(x, view)
+        y.backward(seed)
+    del y
+    grads = [p.grad for p in net.parameters()]
+    for _ in range(3):
+        for t in grads:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, grads))
