@@ -24,8 +24,15 @@ typedef unsigned long long ull;
 constexpr unsigned NONE = 0xffffffffu;
 constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 16, LOW = 255, LOW_TOKENS = 512;
 
-template <typename T, int V> struct Vec { typedef T type __attribute__((ext_vector_type(V))); };
+// V elements at any element-aligned address (global memory takes unaligned vector accesses).  A row of d >= V elements is covered by
+// ceil(d / V) vectors, the last one drawn back to end with the row: what two of them share is the same values twice.
+template <typename T, int V> struct Vec;
+template <> struct Vec<float, 4> { typedef float type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Vec<float, 8> { typedef float type __attribute__((ext_vector_type(8), aligned(4))); };
+template <> struct Vec<_Float16, 8> { typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2))); };
+template <> struct Vec<__bf16, 8> { typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2))); };
 template <typename T> struct Vec<T, 1> { typedef T type; };
+template <int V> __device__ __forceinline__ int column(int c, int d) { return c * V < d - V ? c * V : d - V; }
 template <typename T, int V> __device__ __forceinline__ float at(const typename Vec<T, V>::type& x, int e) {
   if constexpr (V == 1) return (float)x;
   else return (float)x[e];
@@ -41,11 +48,11 @@ __device__ __forceinline__ ll load_index(const void* index, int index64, ll i) {
 
 // one lane per V columns of a row
 template <typename T, int V>
-__global__ __launch_bounds__(256) void lookup_kernel(const void* index, int index64, ll n, ll v, int cols, float scale, const T* __restrict__ table,
+__global__ __launch_bounds__(256) void lookup_kernel(const void* index, int index64, ll n, ll v, int cols, int d, float scale, const T* __restrict__ table,
                                                      ll ldt, T* __restrict__ rows, ll ldr) {
   typedef typename Vec<T, V>::type VT;
   for (ll e = (ll)blockIdx.x * 256 + threadIdx.x; e < n * cols; e += (ll)gridDim.x * 256) {
-    const ll i = e / cols, c = (e % cols) * V;
+    const ll i = e / cols, c = column<V>((int)(e % cols), d);
     const ll k = load_index(index, index64, i);
     VT y = {};
     if (k >= 0 && k < v) {
@@ -243,7 +250,7 @@ template <typename T, int V> __device__ __forceinline__ void clear_rows(const Le
     const VT z = {};
     for (ull todo = __ballot(clear); todo; todo &= todo - 1) {
       T* out = (T*)a.out + (r0 + __builtin_ctzll(todo)) * a.ldo;
-      for (int c = lane; c < a.cols; c += 64) *(VT*)(out + (ll)c * V) = z;
+      for (int c = lane; c < a.cols; c += 64) *(VT*)(out + column<V>(c, a.d)) = z;
     }
   }
 }
@@ -261,7 +268,7 @@ __global__ __launch_bounds__(256) void sum_kernel(const Level a) {
   const int c = blockIdx.y * a.width + threadIdx.x % a.width;
   const ll beg = g * a.run, end = beg + a.run < a.n ? beg + a.run : a.n;
   if (beg >= a.n || c >= a.cols) return;
-  const ll col = (ll)c * V;
+  const ll col = column<V>(c, a.d);
   unsigned cur = NONE;
   bool head = true;              // the run in hand is the group's first
   float acc[V];
@@ -343,88 +350,151 @@ struct Low {
   float* part;                   // [workgroups][v][d]; null: one workgroup, which writes the table
 };
 
-// 512 tokens: counting sort by row in LDS (stable), then a group of lanes per row adds up its tokens
+// 512 tokens: counting sort by row in LDS (stable); then groups of lanes walk equal shares of the sorted tokens.  A run that ends inside a
+// share is done; the first and the last run of a share meet their neighbours' in LDS, where the share in which a run starts adds up the rest.
+// blockIdx.y: 64 vectors of the row each.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void low_kernel(const Low a) {
+__global__ __launch_bounds__(LOW_TOKENS) void low_kernel(const Low a) {
   typedef typename Vec<T, V>::type VT;
   typedef typename Vec<float, V>::type FT;
-  constexpr int ROUNDS = LOW_TOKENS / 256, BATCH = 8;
-  __shared__ unsigned cnt[4][256];
+  constexpr int WAVES = LOW_TOKENS / 64, BATCH = 8, GROUPS = 32;
+  __shared__ unsigned cnt[WAVES][256];
   __shared__ unsigned buf[256];
   __shared__ unsigned start[257];
-  __shared__ unsigned short order[LOW_TOKENS];
+  __shared__ unsigned short order[LOW_TOKENS], sorted[LOW_TOKENS];
+  __shared__ float edge[2 * LOW_TOKENS * V];             // [group][first | last][lane][V]
+  __shared__ unsigned edge_key[2 * GROUPS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  for (int w = 0; w < 4; ++w) cnt[w][tid] = 0;
+  if (tid < 256)
+    for (int w = 0; w < WAVES; ++w) cnt[w][tid] = 0;
   __syncthreads();
-  volatile unsigned* mine = cnt[wave];
   const ll tok0 = (ll)blockIdx.x * LOW_TOKENS;
-  const int first = wave * (LOW_TOKENS / 4);
-  unsigned key[ROUNDS], rank[ROUNDS];
+  const bool live = tok0 + tid < a.n;
+  const unsigned key = live ? key_of(a.index, a.index64, tok0 + tid, a.v) : 0;
+  ull peers = __ballot(live);
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const ll i = tok0 + first + r * 64 + lane;
-    const bool live = i < a.n;
-    key[r] = live ? key_of(a.index, a.index64, i, a.v) : 0;
-    ull peers = __ballot(live);
+  for (int b = 0; b < 8; ++b) {
+    const ull on = __ballot((key >> b) & 1);
+    peers &= (key >> b) & 1 ? on : ~on;
+  }
+  const unsigned before = (unsigned)__popcll(peers & ((1ull << lane) - 1));
+  if (live && before == 0) cnt[wave][key] = (unsigned)__popcll(peers);
+  __syncthreads();
+  unsigned own = 0;
+  if (tid < 256)
+    for (int w = 0; w < WAVES; ++w) own += cnt[w][tid];
+  // exclusive scan of the 256 counts by the first four waves
+  unsigned in = own;
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const ull on = __ballot((key[r] >> b) & 1);
-      peers &= (key[r] >> b) & 1 ? on : ~on;
-    }
-    const unsigned before = (unsigned)__popcll(peers & ((1ull << lane) - 1));
-    if (live) {
-      const unsigned c = mine[key[r]];
-      rank[r] = c + before;
-      if (before == 0) mine[key[r]] = c + (unsigned)__popcll(peers);
+  for (int d = 1; d < 64; d *= 2) {
+    const unsigned y = __shfl_up(in, d);
+    if (lane >= d) in += y;
+  }
+  if (tid < 256 && lane == 63) buf[wave] = in;
+  __syncthreads();
+  if (tid < 256) {
+    unsigned c = in - own + (wave > 0 ? buf[0] : 0) + (wave > 1 ? buf[1] : 0) + (wave > 2 ? buf[2] : 0);
+    start[tid] = c;
+    if (tid == 255) start[256] = c + own;
+    for (int w = 0; w < WAVES; ++w) {
+      const unsigned x = cnt[w][tid];
+      cnt[w][tid] = c;
+      c += x;
     }
   }
   __syncthreads();
-  unsigned own = 0, total;
-  for (int w = 0; w < 4; ++w) own += cnt[w][tid];
-  unsigned c = scan256(own, buf, total);
-  start[tid] = c;
-  if (tid == 255) start[256] = c + own;
-  for (int w = 0; w < 4; ++w) {
-    const unsigned x = cnt[w][tid];
-    cnt[w][tid] = c;
-    c += x;
+  if (live) {
+    const unsigned to = cnt[wave][key] + before;
+    order[to] = (unsigned short)tid;
+    sorted[to] = (unsigned short)key;
   }
   __syncthreads();
+  const int named = (int)start[a.v];                     // tokens that name a row (the others have key v and come last)
+  const int groups = LOW_TOKENS / a.width < GROUPS ? LOW_TOKENS / a.width : GROUPS, share = LOW_TOKENS / groups;
+  const int g = tid / a.width, l = tid % a.width, c = blockIdx.y * a.width + l;
+  const bool on = g < groups && c < a.cols;
+  const ll col = column<V>(c < a.cols ? c : 0, a.d);
+  auto finish = [&](unsigned row, const float* acc) {
+    if (a.part) {
+      FT y;
 #pragma unroll
-  for (int r = 0; r < ROUNDS; ++r)
-    if (tok0 + first + r * 64 + lane < a.n) order[cnt[wave][key[r]] + rank[r]] = (unsigned short)(first + r * 64 + lane);
-  __syncthreads();
-  const int per = 256 / a.width, g = tid / a.width;
-  for (int row = g; row < a.v; row += per) {
-    const unsigned beg = start[row], end = start[row + 1];
-    for (int col = tid % a.width; col < a.cols; col += a.width) {
-      float acc[V];
+      for (int q = 0; q < V; ++q) put<float, V>(y, q, acc[q]);
+      *(FT*)(a.part + ((ll)blockIdx.x * a.v + row) * a.d + col) = y;
+    } else {
+      VT y;
 #pragma unroll
-      for (int q = 0; q < V; ++q) acc[q] = 0.0f;
-      for (unsigned e = beg; e < end; e += BATCH) {
-        VT x[BATCH];
+      for (int q = 0; q < V; ++q) put<T, V>(y, q, a.scale * acc[q]);
+      *(VT*)((T*)a.out + row * a.ldo + col) = y;
+    }
+  };
+  auto keep = [&](int slot, unsigned k, const float* acc) {
+    if (l == 0) edge_key[slot] = k;
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          if (e + b < end) x[b] = *(const VT*)((const T*)a.rows + (tok0 + order[e + b]) * a.ldr + (ll)col * V);
+    for (int q = 0; q < V; ++q) edge[(slot * a.width + l) * V + q] = acc[q];
+  };
+  float acc[V];
 #pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          if (e + b < end) {
+  for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+  if (on) {
+    const int beg = g * share, end = beg + share < named ? beg + share : named;
+    unsigned cur = NONE;
+    bool head = true;
+    for (int e = beg; e < end; e += BATCH) {
+      VT x[BATCH];
 #pragma unroll
-            for (int q = 0; q < V; ++q) acc[q] += at<T, V>(x[b], q);
+      for (int b = 0; b < BATCH; ++b)
+        if (e + b < end) x[b] = *(const VT*)((const T*)a.rows + (tok0 + order[e + b]) * a.ldr + col);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b)
+        if (e + b < end) {
+          const unsigned k = sorted[e + b];
+          if (k != cur) {
+            if (cur != NONE) {
+              if (head) keep(2 * g, cur, acc);
+              else finish(cur, acc);
+              head = false;
+            }
+            cur = k;
+#pragma unroll
+            for (int q = 0; q < V; ++q) acc[q] = 0.0f;
           }
-      }
-      if (a.part) {
-        FT y;
 #pragma unroll
-        for (int q = 0; q < V; ++q) put<float, V>(y, q, acc[q]);
-        *(FT*)(a.part + ((ll)blockIdx.x * a.v + row) * a.d + (ll)col * V) = y;
-      } else {
-        VT y;
-#pragma unroll
-        for (int q = 0; q < V; ++q) put<T, V>(y, q, a.scale * acc[q]);
-        *(VT*)((T*)a.out + row * a.ldo + (ll)col * V) = y;
-      }
+          for (int q = 0; q < V; ++q) acc[q] += at<T, V>(x[b], q);
+        }
     }
+    if (head) {
+      keep(2 * g, cur, acc);
+      if (l == 0) edge_key[2 * g + 1] = NONE;
+    } else {
+      keep(2 * g + 1, cur, acc);
+    }
+  } else if (g < groups && l == 0) {
+    edge_key[2 * g] = edge_key[2 * g + 1] = NONE;        // (lane 0 of a group has a column whenever any lane has)
+  }
+  __syncthreads();
+  if (on) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {                          // (two neighbouring slots of one share never hold the same row)
+      const int slot = 2 * g + h;
+      const unsigned k = edge_key[slot];
+      if (k == NONE || (h == 0 && g > 0 && (edge_key[slot - 1] == k || (edge_key[slot - 1] == NONE && edge_key[slot - 2] == k)))) continue;
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] = edge[(slot * a.width + l) * V + q];
+      for (int s = slot + 1; s < 2 * groups; ++s) {
+        const unsigned ks = edge_key[s];
+        if (ks == NONE) continue;
+        if (ks != k) break;
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] += edge[(s * a.width + l) * V + q];
+      }
+      finish(k, acc);
+    }
+  }
+  if (on) {                                              // rows that none of these tokens names
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+    for (int row = g; row < a.v; row += groups)
+      if (start[row] == start[row + 1]) finish(row, acc);
   }
 }
 
@@ -492,11 +562,9 @@ long long backward_workspace_bytes(long long n, long long v, long long d) {
 // a grid's threads are counted in 32 bits: larger ranges loop
 static dim3 blocks(ll n) { return dim3((unsigned)(n < (1 << 22) ? n : (1 << 22))); }
 
-static bool vec_ok(const void* p, ll ld, ll d, int es) { return (uintptr_t)p % 16 == 0 && (ld * es) % 16 == 0 && (d * es) % 16 == 0; }
-
 template <typename T, int V> static int forward_as(const Call& c, hipStream_t st) {
-  const ll cols = c.d / V;
-  lookup_kernel<T, V><<<blocks((c.n * cols + 255) / 256), 256, 0, st>>>(c.index, c.index64, c.n, c.v, (int)cols, c.scale,
+  const ll cols = (c.d + V - 1) / V;
+  lookup_kernel<T, V><<<blocks((c.n * cols + 255) / 256), 256, 0, st>>>(c.index, c.index64, c.n, c.v, (int)cols, (int)c.d, c.scale,
                                                                                   (const T*)c.src, c.lds, (T*)c.dst, c.ldd);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
@@ -510,7 +578,7 @@ template <typename T, int V> static int low_as(const Call& c, hipStream_t st) {
   a.ldo = c.ldd;
   a.v = (int)c.v;
   a.d = (int)c.d;
-  a.cols = (int)(c.d / V);
+  a.cols = (int)((c.d + V - 1) / V);
   a.width = 1;
   while (a.width < a.cols && a.width < 64) a.width *= 2;
   a.scale = c.scale;
@@ -518,7 +586,7 @@ template <typename T, int V> static int low_as(const Call& c, hipStream_t st) {
   a.out = c.dst;
   const ll parts = c.n > 0 ? low_parts(c.n) : 1;
   a.part = parts > 1 ? (float*)c.ws : nullptr;
-  low_kernel<T, V><<<dim3((unsigned)parts), 256, 0, st>>>(a);
+  low_kernel<T, V><<<dim3((unsigned)parts, (unsigned)((a.cols + a.width - 1) / a.width)), LOW_TOKENS, 0, st>>>(a);
   if (parts > 1) low_join_kernel<T><<<dim3((unsigned)((c.v * c.d + 63) / 64)), 1024, 0, st>>>(a, (int)parts);
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
@@ -527,7 +595,7 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
   const ll need = backward_workspace_bytes(c.n, c.v, c.d);
   if (need > 0 && (!c.ws || c.ws_bytes < need)) return -3;
   if (low(c.n, c.v, c.d)) return low_as<T, V>(c, st);
-  const int cols = (int)(c.d / V);
+  const int cols = (int)((c.d + V - 1) / V);
   const Layout l = layout(c.n, c.d);
   char* ws = (char*)c.ws;
   unsigned *keys[2], *perm[2];
@@ -595,16 +663,14 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
 }
 
 int forward(const Call& c, hipStream_t st) {
-  const int es = c.dtype == nrhlin::F32 ? 4 : 2;
-  const bool vec = vec_ok(c.src, c.lds, c.d, es) && vec_ok(c.dst, c.ldd, c.d, es);
+  const bool vec = c.d >= (c.dtype == nrhlin::F32 ? 4 : 8);      // rows of at least 16 bytes
   if (c.dtype == nrhlin::F32) return vec ? forward_as<float, 4>(c, st) : forward_as<float, 1>(c, st);
   if (c.dtype == nrhlin::F16) return vec ? forward_as<_Float16, 8>(c, st) : forward_as<_Float16, 1>(c, st);
   return vec ? forward_as<__bf16, 8>(c, st) : forward_as<__bf16, 1>(c, st);
 }
 
 int backward(const Call& c, hipStream_t st) {
-  const int es = c.dtype == nrhlin::F32 ? 4 : 2;
-  const bool vec = vec_ok(c.src, c.lds, c.d, es) && vec_ok(c.dst, c.ldd, c.d, es);
+  const bool vec = c.d >= (c.dtype == nrhlin::F32 ? 4 : 8);      // rows of at least 16 bytes
   if (c.dtype == nrhlin::F32) return vec ? backward_as<float, 4>(c, st) : backward_as<float, 1>(c, st);
   if (c.dtype == nrhlin::F16) return vec ? backward_as<_Float16, 8>(c, st) : backward_as<_Float16, 1>(c, st);
   return vec ? backward_as<__bf16, 8>(c, st) : backward_as<__bf16, 1>(c, st);

@@ -74,6 +74,10 @@ template <typename X> struct Chunk {
 #pragma unroll
     for (int e = 4; e < W; ++e) w[e] = 0;
   }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < W; ++e) w[e] = 0;
+  }
   // the 8 elements behind p moved down by k (0 .. 8): p + k .. and zeros
   __device__ __forceinline__ void drop(int k) {
     constexpr int PER = 4 / sizeof(X);                 // elements per word
@@ -158,6 +162,28 @@ __device__ __forceinline__ float exp_minus(float a) {
   return __builtin_amdgcn_exp2f(-h) * fmaf(l, -0.693147182f, 1.0f);
 }
 
+// log(1 + e), 0 <= e <= 1: a series below 1/64 (the next term is under 2^-26 of it), above it log(u) e / (u - 1) of the rounded u = 1 + e
+__device__ __forceinline__ float log1p_unit(float e) {
+  if (e < 0.015625f) return e * (1.0f - e * (0.5f - e * (0.333333343f - e * 0.25f)));
+  const float u = 1.0f + e;
+  return 0.693147182f * __builtin_amdgcn_logf(u) * (e * __builtin_amdgcn_rcpf(u - 1.0f));
+}
+
+// erfc(x), 0 <= x <= 14, as e^(-x^2) t P(t), t = 1 / (1 + x / 2): P is the polynomial of degree 8 with the least relative error over
+// that range (4.5e-8, by reweighted least squares on Chebyshev nodes in float64; 5.6 2^-24 as evaluated here).  ex2: e^(-x^2).
+__device__ __forceinline__ float erfc_positive(float x, float ex2) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
+  float q = fmaf(t, -0.05938727781f, 0.28612756729f);
+  q = fmaf(t, q, -0.49041295052f);
+  q = fmaf(t, q, 0.28173971176f);
+  q = fmaf(t, q, -0.02915211208f);
+  q = fmaf(t, q, 0.20375365019f);
+  q = fmaf(t, q, 0.24283494055f);
+  q = fmaf(t, q, 0.28241211176f);
+  q = fmaf(t, q, 0.28208434582f);
+  return ex2 * (t * q);
+}
+
 // act(z) and act'(z); every exponential has a non-positive argument, so none overflows, and NaN passes through
 __device__ __forceinline__ float act_eval(int act, float beta, float z, float& d) {
   if (act == NONE) { d = 1.0f; return z; }
@@ -166,11 +192,13 @@ __device__ __forceinline__ float act_eval(int act, float beta, float z, float& d
     const float e = exp_minus(fabsf(beta * z));
     const float s = __builtin_amdgcn_rcpf(1.0f + e);
     d = z != z ? z : (z > 0.0f ? s : e * s);
-    return (z < 0.0f ? 0.0f : z) + log1pf(e) / beta;
+    return (z < 0.0f ? 0.0f : z) + log1p_unit(e) * __builtin_amdgcn_rcpf(beta);
   }
-  if (act == GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * z);      // erfc: no cancellation for negative z
-    d = phi + z * (0.3989422804014327f * exp_minus(0.5f * z * z));
+  if (act == GELU) {                                   // z Phi(z), Phi(z) = erfc(-z / sqrt 2) / 2
+    const float x = fminf(fabsf(z) * 0.70710678118654752f, 14.0f), s = x * x;
+    const float ex2 = exp_minus(s) * (1.0f - fmaf(x, x, -s));
+    const float half = 0.5f * erfc_positive(x, ex2), phi = z < 0.0f ? half : 1.0f - half;
+    d = phi + z * (0.3989422804014327f * ex2);
     return z * phi;
   }
   const float e = exp_minus(fabsf(z));
@@ -357,32 +385,50 @@ template <typename X, int N> __device__ __forceinline__ void store(X* p, const f
   }
 }
 
-// 32 x COLS_ finished values of one wave, wholly inside the output.  MODE: an activation (FORWARD), STORE (as they are) or RAW
-// (float32 partial sums).
+template <typename X, int N> __device__ __forceinline__ void put(X* p, const float* x, int left) {      // ... the first `left` of them
+  if (left >= N) store<X, N>(p, x);
+  else {
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (e < left) p[e] = (X)x[e];
+  }
+}
+
+// 32 x COLS_ finished values of one wave, of which rows x cols lie in the output.  MODE: an activation (FORWARD), STORE (as they are) or
+// RAW (float32 partial sums).
 enum Mode { STORE = 16, RAW = 17 };
 template <typename T, int COLS_, int EPITCH, int MODE>
-__device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const float* ep, ll i0, ll j0, int lane) {
+__device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const float* ep, ll i0, ll j0, int rows, int cols, int lane) {
   constexpr int C = MODE == RAW || sizeof(T) == 4 ? 4 : 8, LPR = COLS_ / C, RPI = 64 / LPR, UN = 4;
-  const int col = C * (lane % LPR), row0 = lane / LPR;
+  constexpr int IT = 32 / RPI, U = IT < UN ? IT : UN;
+  const int col = C * (lane % LPR), row0 = lane / LPR, left = cols - col;      // columns of this lane that exist
+  if (left <= 0) return;
   const ll j = j0 + col;
   float b[C];
 #pragma unroll
   for (int e = 0; e < C; ++e) b[e] = 0.0f;
   if (MODE < STORE && a.bias) {
 #pragma unroll
-    for (int e = 0; e < C; ++e) b[e] = (float)((const T*)a.bias)[j + e];
+    for (int e = 0; e < C; ++e)
+      if (e < left) b[e] = (float)((const T*)a.bias)[j + e];
   }
-  constexpr int IT = 32 / RPI, U = IT < UN ? IT : UN;
 #pragma unroll 1
   for (int it = 0; it < IT; it += U) {
     Chunk<T> r[U];                                     // C elements of the residual (float32: the first half)
     if constexpr (MODE < STORE) if (a.res) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) r[u].load_16((const T*)a.res + (i0 + row0 + (it + u) * RPI) * a.ldr + j);
+      for (int u = 0; u < U; ++u) {
+        const int row = row0 + (it + u) * RPI;
+        const T* p = (const T*)a.res + (i0 + row) * a.ldr + j;
+        if (row >= rows) r[u].zero();
+        else if (left >= C) r[u].load_16(p);
+        else r[u].load_single(p, left);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int row = row0 + (it + u) * RPI;
+      if (row >= rows) break;
       const ll i = i0 + row;
       float z[C], d[C], f[8];
 #pragma unroll
@@ -391,7 +437,7 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
 #pragma unroll
         for (int e = 0; e < 4; ++e) z[h + e] = x[e];
       }
-      if constexpr (MODE == RAW) store<float, C>((float*)out + i * ldo + j, z);
+      if constexpr (MODE == RAW) put<float, C>((float*)out + i * ldo + j, z, left);
       else {
         if constexpr (MODE < STORE) {
           if (a.res) r[u].floats(f);
@@ -401,11 +447,11 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
             if (a.res) z[e] += f[e];
           }
           if (a.dact && MODE != NONE) {
-            if constexpr (MODE == RELU) store<T, C>((T*)a.dact + i * a.J + j, d);
-            else store<typename Ty<T>::D, C>((typename Ty<T>::D*)a.dact + i * a.J + j, d);
+            if constexpr (MODE == RELU) put<T, C>((T*)a.dact + i * a.J + j, d, left);
+            else put<typename Ty<T>::D, C>((typename Ty<T>::D*)a.dact + i * a.J + j, d, left);
           }
         }
-        store<T, C>((T*)out + i * ldo + j, z);
+        put<T, C>((T*)out + i * ldo + j, z, left);
       }
     }
   }
@@ -433,7 +479,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
   typedef Stage<T, SJ, PLAIN, true, BJ, BK, NT, SINGLE> StJ;
   extern __shared__ __align__(16) char lds[];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
   // consecutive tiles (same A rows) go to one XCD: workgroups are dealt to the 8 XCDs in turn, and each has its own L2
   const unsigned total = gridDim.x, per = total / 8, rem = total % 8, xcd = blockIdx.x % 8;
   unsigned t = xcd * per + (xcd < rem ? xcd : rem) + blockIdx.x / 8;
@@ -461,7 +507,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     else sj.template piece<false>(q - StI::PIECES, px, py, b + PL * StI::Tl::BYTES, nullptr, tid);
   };
 
-  const int wi = wave / WJ, wj = wave % WJ;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
   f32x16 acc[NI][NJ] = {};
   constexpr int READS = (NI + NJ) * PL, MF = NI * NJ * (PL == 3 ? 6 : 1);      // per 16 values of the reduction
   constexpr int PUT0 = KK > 2 ? KK - 3 : 0, PUTS = KK - 1 - PUT0;              // the sixteens beside which the next step goes to LDS
@@ -579,10 +625,23 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     }
   }
 
+  if (OP == BACK_WEIGHT && a.bias_bar && tj == 0) {    // bbar: the threads that share 8 columns
+    float* fl = (float*)lds;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) fl[(tid / StI::CW) * BI + 8 * (tid % StI::CW) + e] = bs[e];
+    __syncthreads();
+    if (tid < BI && i0 + tid < a.I) {
+      float x = 0.0f;
+      for (int c = 0; c < NT / StI::CW; ++c) x += fl[c * BI + tid];
+      if (a.part) a.part_bias[s * a.I + i0 + tid] = x;
+      else ((T*)a.bias_bar)[i0 + tid] = (T)x;
+    }
+  }
+
   // the tile leaves through LDS, 32 rows of a wave at a time: a lane then finishes 16 bytes of a row, and rows are stored in whole
   // cache lines
   float* ep = (float*)lds + wave * 32 * EPITCH;
-  const bool inside = i0 + BI <= a.I && j0 + BJ <= a.J;
   const ll jw = j0 + wj * NJ * 32;
 #pragma unroll 1
   for (int x = 0; x < NI; ++x) {
@@ -599,44 +658,15 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
       }
     __syncthreads();
     const ll iw = i0 + (wi * NI + x) * 32;
-    if (inside) {
-      if (a.part) emit<T, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, lane);
-      else if (OP != FORWARD) emit<T, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else if (a.act == NONE) emit<T, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else if (a.act == RELU) emit<T, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else if (a.act == SOFTPLUS) emit<T, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else if (a.act == SIGMOID) emit<T, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else if (a.act == SILU) emit<T, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, lane);
-      else emit<T, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, lane);
-    } else {                                           // a tile at an edge: one element per lane
-      const int rows = a.I - iw < 32 ? (int)(a.I - iw) : 32, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
-      for (int e = lane; e < rows * cols && cols > 0; e += 64) {
-        const int row = e / cols, col = e % cols;
-        const ll i = iw + row, j = jw + col;
-        float z = ep[row * EPITCH + col], d;
-        if (a.part) {
-          a.part[(s * a.I + i) * a.J + j] = z;
-          continue;
-        }
-        if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
-        ((T*)a.out)[i * a.ldo + j] = (T)z;
-        if (OP == FORWARD && a.dact) keep<T>(a, i * a.J + j, d);
-      }
-    }
-  }
-
-  if (OP == BACK_WEIGHT && a.bias_bar && tj == 0) {    // bbar: the threads that share 8 columns
-    float* fl = (float*)lds;
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 8; ++e) fl[(tid / StI::CW) * BI + 8 * (tid % StI::CW) + e] = bs[e];
-    __syncthreads();
-    if (tid < BI && i0 + tid < a.I) {
-      float x = 0.0f;
-      for (int c = 0; c < NT / StI::CW; ++c) x += fl[c * BI + tid];
-      if (a.part) a.part_bias[s * a.I + i0 + tid] = x;
-      else ((T*)a.bias_bar)[i0 + tid] = (T)x;
-    }
+    const int rows = a.I - iw < 32 ? (int)(a.I - iw) : 32, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
+    if (a.part) emit<T, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, rows, cols, lane);
+    else if (OP != FORWARD) emit<T, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else if (a.act == NONE) emit<T, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else if (a.act == RELU) emit<T, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else if (a.act == SOFTPLUS) emit<T, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else if (a.act == SIGMOID) emit<T, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else if (a.act == SILU) emit<T, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    else emit<T, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
   }
 }
 
@@ -735,8 +765,7 @@ struct Plan {
   ll TI, TJ, chunk;
 };
 
-// The variant with the least tile area per unit of rate, in whole rounds over 256 CUs, and how many splits of the reduction fill
-// them.  The 256 x 256 tile of the 16-bit types has no registers left for act' beside it.
+// The variant with the least tile area per unit of rate, in whole rounds over 256 CUs, and how many splits of the reduction fill them.
 static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
   const int CHUNK = 64;                                 // a multiple of every variant's step
   Plan p = {};
@@ -754,8 +783,12 @@ static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
   else {
     float best = 0.0f;
     for (int v = SMALL; v <= LARGE; ++v) {
-      if ((v == MIDDLE && dtype == F32) || (v == LARGE && dtype != F32 && op != FORWARD && act != NONE)) continue;
-      const Size z = size_of(dtype, v);
+      if (v == MIDDLE && dtype == F32) continue;
+      Size z = size_of(dtype, v);
+      if (v == LARGE && dtype != F32 && op != FORWARD && act != NONE) {
+        if (op == BACK_WEIGHT && I <= z.bi && J <= z.bj) continue;     // (one tile: 62 us against 55 at m = 163840, k = n = 256)
+        z.rate = 0.85f;                                                // its steps are half as long
+      }
       const ll n = tiles(v) * splits(v);
       const float rounds = n > 2048 ? n / 256.0f : (float)((n + 255) / 256);
       const float cost = rounds * z.i * z.j / z.rate / splits(v);
@@ -810,8 +843,7 @@ template <typename T, int OP, int DM> static int start_tile(const Args& a, int v
     return start<T, OP, DM, 4, 2, 2, 2, 32, 2>(a, grid, st);
   } else {
     if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 64, 2>(a, grid, st);
-    if constexpr (DM == PLAIN)
-      if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, 64, 2>(a, grid, st);
+    if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, DM == PLAIN ? 64 : 32, 2>(a, grid, st);      // (act' takes registers)
     return start<T, OP, DM, 2, 2, 2, 2, 64, 2>(a, grid, st);
   }
 }
