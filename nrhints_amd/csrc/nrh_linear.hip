@@ -786,7 +786,7 @@ static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
       if (v == MIDDLE && dtype == F32) continue;
       Size z = size_of(dtype, v);
       if (v == LARGE && dtype != F32 && op != FORWARD && act != NONE) {
-        if (op == BACK_WEIGHT && I <= z.bi && J <= z.bj) continue;     // (one tile: 62 us against 55 at m = 163840, k = n = 256)
+        if (op == BACK_WEIGHT && I <= z.i && J <= z.j) continue;     // (one tile: 62 us against 55 at m = 163840, k = n = 256)
         z.rate = 0.85f;                                                // its steps are half as long
       }
       const ll n = tiles(v) * splits(v);
