@@ -94,6 +94,15 @@ template <typename X> struct Chunk {
       for (int e = 0; e < W; ++e) w[e] = on ? (w[e] >> 16 | (e + 1 < W ? w[e + 1] << 16 : 0u)) : w[e];
     }
   }
+  // the first k (0 .. 8) elements and zeros
+  __device__ __forceinline__ void first(int k) {
+    constexpr int PER = 4 / sizeof(X);
+#pragma unroll
+    for (int e = 0; e < W; ++e) {
+      const int have = k - PER * e;
+      w[e] = have >= PER ? w[e] : (PER == 2 && have == 1 ? w[e] & 0xffffu : 0u);
+    }
+  }
   // the same one by one, for tensors too small to hold 8 elements before the end
   __device__ __forceinline__ void load_single(const X* p, ll n) {
 #pragma unroll
@@ -247,8 +256,8 @@ template <typename L8, int SRC, int BA, int BK, bool PERM> __device__ __forceinl
 template <typename T, int DM> struct Factor { typedef typename Ty<T>::D type; };
 template <typename T> struct Factor<T, MASK> { typedef T type; };
 
-// One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: the tensors may hold fewer than
-// 8 elements before an end (reductions shorter than 8, or a tiny tensor).
+// One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: a tensor may hold fewer than
+// 16 elements.
 template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool SINGLE> struct Stage {
   typedef typename Factor<T, DM>::type Q;
   typedef typename Ty<T>::L L;
@@ -271,7 +280,9 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool S
     } else {
       // (addresses are worked out here, every time: moved out of the loop they would hold dozens of registers)
       asm volatile("" : "+v"(tid));
-      int gone[NC];                                     // a chunk at an end: the last 8 elements, and so many of them dropped
+      // a chunk at an end: the tensor's last 8 elements, and so many of them dropped; a short row's, when others follow: loaded on
+      // into the next row, and all but so many cut off (below zero)
+      int some = 0, gone[NC];
 #pragma unroll
       for (int u = 0; u < NC; ++u) {
         const int row = tid / ROW + u * STEP, col = 8 * (tid % ROW);
@@ -287,17 +298,23 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool S
           at = p + r * ld + a;
           left = r < rn && a < n ? (R - 1 - r) * ld + n - a : 0;      // past the row's end lies the next row, up to the tensor's end
         }
+        const bool any = SRC == COLS && r < rn && a >= n;              // columns past n: any values
+
         if (SINGLE) c[u].load_single(at, left);
         else {
-          gone[u] = left >= 8 ? 0 : (left <= 0 ? 8 : 8 - (int)left);
-          c[u].load(left <= 0 ? p : at - gone[u]);
+          gone[u] = left >= 8 || any ? 0 : (left <= 0 ? 8 : 8 - (int)left);
+          some |= gone[u];
+          const bool on = SRC == ROWS && left < 8 && at + 8 <= p + (n - 1) * ld + R;
+          c[u].load(left <= 0 ? p : at - (on ? 0 : gone[u]));
+          if (on && left > 0) gone[u] = -(int)left;
         }
         __builtin_amdgcn_sched_barrier(0);               // addresses one after another: this is not the path to hold registers for
       }
-      if (!SINGLE) {
+      if (!SINGLE && __ballot(some != 0)) {              // (dropping waits for the loads: only where an end is in reach)
 #pragma unroll
         for (int u = 0; u < NC; ++u) {
-          c[u].drop(gone[u]);
+          c[u].drop(gone[u] > 0 ? gone[u] : 0);
+          if (SRC == ROWS) c[u].first(gone[u] < 0 ? -gone[u] : 8);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
@@ -395,13 +412,13 @@ template <typename X, int N> __device__ __forceinline__ void put(X* p, const flo
 }
 
 // 32 x COLS_ finished values of one wave, of which rows x cols lie in the output.  MODE: an activation (FORWARD), STORE (as they are) or
-// RAW (float32 partial sums).
+// RAW (float32 partial sums).  WHOLE: all do, and nothing is asked per row (655 360 x 256 x 256 bf16 with a residual: 215 us against 247).
 enum Mode { STORE = 16, RAW = 17 };
-template <typename T, int COLS_, int EPITCH, int MODE>
+template <typename T, int COLS_, int EPITCH, int MODE, bool WHOLE>
 __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const float* ep, ll i0, ll j0, int rows, int cols, int lane) {
   constexpr int C = MODE == RAW || sizeof(T) == 4 ? 4 : 8, LPR = COLS_ / C, RPI = 64 / LPR, UN = 4;
   constexpr int IT = 32 / RPI, U = IT < UN ? IT : UN;
-  const int col = C * (lane % LPR), row0 = lane / LPR, left = cols - col;      // columns of this lane that exist
+  const int col = C * (lane % LPR), row0 = lane / LPR, left = WHOLE ? C : cols - col;      // columns of this lane that exist
   if (left <= 0) return;
   const ll j = j0 + col;
   float b[C];
@@ -416,19 +433,23 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
   for (int it = 0; it < IT; it += U) {
     Chunk<T> r[U];                                     // C elements of the residual (float32: the first half)
     if constexpr (MODE < STORE) if (a.res) {
+      const T* p = (const T*)a.res + (i0 + row0 + it * RPI) * a.ldr + j;
+      if (WHOLE) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int row = row0 + (it + u) * RPI;
-        const T* p = (const T*)a.res + (i0 + row) * a.ldr + j;
-        if (row >= rows) r[u].zero();
-        else if (left >= C) r[u].load_16(p);
-        else r[u].load_single(p, left);
+        for (int u = 0; u < U; ++u) r[u].load_16(p + u * RPI * a.ldr);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (row0 + (it + u) * RPI >= rows) r[u].zero();
+          else if (left >= C) r[u].load_16(p + u * RPI * a.ldr);
+          else r[u].load_single(p + u * RPI * a.ldr, left);
+        }
       }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int row = row0 + (it + u) * RPI;
-      if (row >= rows) break;
+      if (!WHOLE && row >= rows) break;
       const ll i = i0 + row;
       float z[C], d[C], f[8];
 #pragma unroll
@@ -659,14 +680,19 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     __syncthreads();
     const ll iw = i0 + (wi * NI + x) * 32;
     const int rows = a.I - iw < 32 ? (int)(a.I - iw) : 32, cols = a.J - jw < 32 * NJ ? (int)(a.J - jw) : 32 * NJ;
-    if (a.part) emit<T, 32 * NJ, EPITCH, RAW>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, rows, cols, lane);
-    else if (OP != FORWARD) emit<T, 32 * NJ, EPITCH, STORE>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else if (a.act == NONE) emit<T, 32 * NJ, EPITCH, NONE>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else if (a.act == RELU) emit<T, 32 * NJ, EPITCH, RELU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else if (a.act == SOFTPLUS) emit<T, 32 * NJ, EPITCH, SOFTPLUS>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else if (a.act == SIGMOID) emit<T, 32 * NJ, EPITCH, SIGMOID>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else if (a.act == SILU) emit<T, 32 * NJ, EPITCH, SILU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
-    else emit<T, 32 * NJ, EPITCH, GELU>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    auto leave = [&](auto WHOLE) {
+      constexpr bool W = WHOLE;
+      if (a.part) emit<T, 32 * NJ, EPITCH, RAW, W>(a, a.part + s * a.I * a.J, a.J, ep, iw, jw, rows, cols, lane);
+      else if (OP != FORWARD) emit<T, 32 * NJ, EPITCH, STORE, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else if (a.act == NONE) emit<T, 32 * NJ, EPITCH, NONE, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else if (a.act == RELU) emit<T, 32 * NJ, EPITCH, RELU, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else if (a.act == SOFTPLUS) emit<T, 32 * NJ, EPITCH, SOFTPLUS, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else if (a.act == SIGMOID) emit<T, 32 * NJ, EPITCH, SIGMOID, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else if (a.act == SILU) emit<T, 32 * NJ, EPITCH, SILU, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+      else emit<T, 32 * NJ, EPITCH, GELU, W>(a, a.out, a.ldo, ep, iw, jw, rows, cols, lane);
+    };
+    if (rows == 32 && cols == 32 * NJ) leave(Const<1>());
+    else leave(Const<0>());
   }
 }
 
@@ -716,95 +742,132 @@ __global__ __launch_bounds__(256) void few_kernel(const Args a) {
   }
 }
 
-// joins the S partial outputs in a fixed order and finishes them like the tile kernel: 64 elements per workgroup, each as 4 sums over
-// every 4th part
-template <typename T, int OP>
+// Joins the S partial outputs in a fixed order and finishes them like the tile kernel: 4 elements per thread, each as SLICES sums over
+// every SLICES-th part (a thread's loads come in turns of 8, each a trip to memory: 67 x 6 elements of 512
+// parts take 48 us with the product on 64 slices and 58 on 16, 256 x 256 elements of 256 parts 77 and 63).  Bound by reading the parts.
+template <typename T, int OP, int SLICES>
 __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
-  __shared__ float buf[4][64];
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  const ll n = a.I * a.J, extra = OP == BACK_WEIGHT && a.bias_bar ? a.I : 0;
-  const ll e = (ll)blockIdx.x * 64 + lane;
-  float z = 0.0f;
-  if (e < n + extra) {
-    const float* p = e < n ? a.part + e : a.part_bias + (e - n);
-    const ll step = e < n ? n : a.I;
+  constexpr int LANES = 256 / SLICES;
+  __shared__ f32x4 buf[SLICES][LANES];
+  const int lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
+  const ll n = a.I * a.J, extra = OP == BACK_WEIGHT && a.bias_bar ? a.I : 0, groups = (n + 3) / 4;
+  const ll g = (ll)blockIdx.x * LANES + lane;
+  const bool main = g < groups;
+  const ll e = 4 * (main ? g : g - groups), step = main ? n : a.I, left = (main ? n : extra) - e;
+  f32x4 z = {};
+  if (left > 0) {
+    typedef float V __attribute__((ext_vector_type(4), aligned(4)));
+    const float* p = (main ? a.part : a.part_bias) + e;
+    if (left >= 4) {
 #pragma unroll 8
-    for (int s = slice; s < a.S; s += 4) z += p[s * step];
+      for (int s = slice; s < a.S; s += SLICES) {
+        const V x = *(const V*)(p + s * step);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[q] += x[q];
+      }
+    } else {
+      for (int s = slice; s < a.S; s += SLICES)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < left) z[q] += p[s * step + q];
+    }
   }
-  buf[slice][lane] = z;
-  __syncthreads();
-  if (slice != 0 || e >= n + extra) return;
-  z = buf[0][lane] + buf[1][lane] + buf[2][lane] + buf[3][lane];
-  if (e >= n) {
-    ((T*)a.bias_bar)[e - n] = (T)z;
+  if (SLICES > 1) {
+    buf[slice][lane] = z;
+    __syncthreads();
+    if (slice != 0) return;
+    for (int s = 1; s < SLICES; ++s)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) z[q] += buf[s][lane][q];
+  }
+  if (left <= 0) return;
+  if (!main) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < left) ((T*)a.bias_bar)[e + q] = (T)z[q];
     return;
   }
-  const ll i = e / a.J, j = e % a.J;
-  float d = 0.0f;
-  if (OP == FORWARD) z = finish<T>(a, i, j, z, d);
-  ((T*)a.out)[i * a.ldo + j] = (T)z;
-  if (OP == FORWARD && a.dact) keep<T>(a, e, d);
+  ll i = e / a.J, j = e % a.J;
+  const bool row = j + 4 <= a.J;                       // one row's: a single store
+  float y[4], d[4];
+  ll at[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    at[q] = i * a.ldo + j;
+    y[q] = z[q];
+    if (OP == FORWARD && q < left) y[q] = finish<T>(a, i, j, z[q], d[q]);
+    if (++j == a.J) { j = 0; ++i; }
+  }
+  if (row) store<T, 4>((T*)a.out + at[0], y);
+  else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < left) ((T*)a.out)[at[q]] = (T)y[q];
+  }
+  if (OP == FORWARD && a.dact) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < left) keep<T>(a, e + q, d[q]);
+  }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------
-// Tile variants: rows x columns, workgroups that fit on a CU, and the rate per area at long reductions (8 192 x 4 096 x 4 096 bf16: 64 x 64
-// 480, 128 x 128 880, 256 x 256 1 180 TFLOP/s; 8 192 x 2 048 x 2 048 f32: 64 x 64 130, 256 x 128 212).
+// Tile variants: rows x columns of the output.  Long reductions reach (8 192 x 4 096 x 4 096 bf16) 480, 880 and 1 180 TFLOP/s on SMALL,
+// MIDDLE and LARGE, (8 192 x 2 048 x 2 048 f32) 130 and 212 on SMALL and LARGE; small outputs want many small tiles.
 enum Variant { FEW = 0, TINY, SMALL, MIDDLE, LARGE };
-struct Size {
-  int i, j, per_cu;
-  float rate;
-};
+struct Size { int i, j; };
 static Size size_of(int dtype, int v) {
-  if (v <= SMALL) return {64, 64, 3, dtype == F32 ? 0.6f : 0.4f};
-  if (v == MIDDLE) return {128, 128, 2, 0.75f};         // 16-bit types
-  return dtype == F32 ? Size{256, 128, 1, 1.0f} : Size{256, 256, 1, 1.0f};
+  if (v <= SMALL) return {64, 64};
+  if (v == MIDDLE) return {128, 128};                   // 16-bit types
+  return dtype == F32 ? Size{256, 128} : Size{256, 256};
 }
+
+// What a launch takes, in microseconds, with w tiles per CU that each reduce L values: start + L max(alone, w each) + (w - 1) tile; and
+// S > 1 splits' parts: JOIN + I J (S PART + LAST).  Fitted (rms 12 %) to 600 timings of 20 shapes from 64 x 1 024 x 1 024 to
+// 400 000 x 256 x 256, every variant at 1 to 256 splits; the choice by it is on average 2 % above the best of each.
+struct Cost { float start, alone, each, tile; };
+static Cost cost_of(int dtype, bool act_bar, int v) {
+  if (v == TINY) return {4.0f, 0.036f, 0.006f, 0.30f};
+  if (dtype == F32) return v <= SMALL ? Cost{4.0f, 0.0234f, 0.0156f, 0.31f} : Cost{7.9f, 0.0388f, 0.0644f, 7.6f};
+  if (v <= SMALL) return act_bar ? Cost{3.6f, 0.0109f, 0.0065f, 0.18f} : Cost{3.4f, 0.0092f, 0.0042f, 0.46f};
+  if (v == MIDDLE) return act_bar ? Cost{5.6f, 0.0121f, 0.0164f, 0.60f} : Cost{5.75f, 0.0011f, 0.0121f, 0.89f};
+  return act_bar ? Cost{8.3f, 0.0093f, 0.0343f, 7.2f} : Cost{8.2f, 0.0040f, 0.0295f, 7.1f};
+}
+constexpr float JOIN = 3.24f, PART = 1.07e-6f, LAST = 1.1e-7f;
 
 struct Plan {
   int variant, S;
   ll TI, TJ, chunk;
 };
 
-// The variant with the least tile area per unit of rate, in whole rounds over 256 CUs, and how many splits of the reduction fill them.
+// the variant and the number of splits with the least cost
 static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
-  const int CHUNK = 64;                                 // a multiple of every variant's step
+  const int CHUNK = 64, MOST = 1024;                    // CHUNK: a multiple of every variant's step
   Plan p = {};
   p.S = 1;
   if (op == FORWARD && I <= 8) return p;                // FEW
-  auto tiles = [&](int v) { return ((I + size_of(dtype, v).i - 1) / size_of(dtype, v).i) * ((J + size_of(dtype, v).j - 1) / size_of(dtype, v).j); };
-  const ll longest = R / (dtype == F32 ? 128 : 256) < 1 ? 1 : R / (dtype == F32 ? 128 : 256);      // splits that leave each some work
-  auto splits = [&](int v) {
-    const ll n = tiles(v) < 1 ? 1 : tiles(v), want = 256 * size_of(dtype, v).per_cu;
-    ll s = n * 2 > want ? 1 : want / n;
-    s = s < longest ? s : longest;
-    return s > 512 ? 512 : s;
-  };
-  if (R < 8 || I < 8 || J < 8) p.variant = TINY;        // an operand may hold fewer than 8 elements before its end: loaded one by one
-  else {
-    float best = 0.0f;
-    for (int v = SMALL; v <= LARGE; ++v) {
-      if (v == MIDDLE && dtype == F32) continue;
-      Size z = size_of(dtype, v);
-      if (v == LARGE && dtype != F32 && op != FORWARD && act != NONE) {
-        if (op == BACK_WEIGHT && I <= z.i && J <= z.j) continue;     // (one tile: 62 us against 55 at m = 163840, k = n = 256)
-        z.rate = 0.85f;                                                // its steps are half as long
-      }
-      const ll n = tiles(v) * splits(v);
-      const float rounds = n > 2048 ? n / 256.0f : (float)((n + 255) / 256);
-      const float cost = rounds * z.i * z.j / z.rate / splits(v);
-      if (p.variant == FEW || cost < best) {
-        p.variant = v;
-        best = cost;
+  const bool act_bar = op != FORWARD && act != NONE;
+  const ll steps = R > 0 ? (R + CHUNK - 1) / CHUNK : 1; // R = 0: the gradient of no rows, one pass over nothing
+  // Loaded one by one: operands of less than two chunks, reductions that end inside the first chunk (305 747 x 2 x 20 bf16 16 us against
+  // 24) and columns that do (the weight gradient of 510 170 x 50 x 3 f16 34 us against 41: chunks would read on into the rows behind).
+  const bool tiny = R < 8 || I * R < 16 || J * R < 16 || (op != FORWARD && J < 8) || (op == BACK_WEIGHT && I < 8);
+  float best = 0.0f;
+  for (int v = tiny ? TINY : SMALL; v <= (tiny ? TINY : LARGE); ++v) {
+    if (v == MIDDLE && dtype == F32) continue;
+    const Size z = size_of(dtype, v);
+    const Cost c = cost_of(dtype, act_bar, v);
+    const ll TI = (I + z.i - 1) / z.i, TJ = (J + z.j - 1) / z.j;
+    for (int s = 1; s <= MOST && s <= steps; s = s < 4 ? s + 1 : s + (s & (s - 1) ? s / 3 : s / 2)) {      // 1 2 3 4 6 8 12 16 ..
+      const ll chunk = (steps + s - 1) / s, S = (steps + chunk - 1) / chunk, n = TI * TJ * S;
+      const float w = n > 2048 ? n / 256.0f : (float)((n + 255) / 256);
+      const float each = c.each * w;
+      const float t = c.start + chunk * CHUNK * (each > c.alone ? each : c.alone) + (w - 1) * c.tile + (S > 1 ? JOIN + (float)I * J * (S * PART + LAST) : 0);
+      if (p.variant == FEW || t < best) {
+        best = t;
+        p = {v, (int)S, TI, TJ, chunk * CHUNK};
       }
     }
   }
-  const Size z = size_of(dtype, p.variant);
-  p.chunk = ((R + splits(p.variant) - 1) / splits(p.variant) + CHUNK - 1) / CHUNK * CHUNK;
-  if (p.chunk < CHUNK) p.chunk = CHUNK;                 // R = 0: the gradient of no rows, one pass over nothing
-  p.S = (int)((R + p.chunk - 1) / p.chunk);
-  if (p.S < 1) p.S = 1;
-  p.TI = (I + z.i - 1) / z.i;
-  p.TJ = (J + z.j - 1) / z.j;
   return p;
 }
 
@@ -901,8 +964,11 @@ static int run(const Call& c, hipStream_t st) {
                                                                                           : start_tile<T, OP, SMOOTH>(a, p.variant, grid, st));
   if (rc) return rc;
   if (p.S > 1) {
-    const ll n = a.I * a.J + (a.bias_bar ? a.I : 0);
-    reduce_kernel<T, OP><<<dim3((unsigned)((n + 63) / 64)), 256, 0, st>>>(a);
+    const ll n = (a.I * a.J + 3) / 4 + (a.bias_bar ? (a.I + 3) / 4 : 0);
+    if (p.S < 8) reduce_kernel<T, OP, 1><<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>(a);
+    else if (p.S < 32) reduce_kernel<T, OP, 4><<<dim3((unsigned)((n + 63) / 64)), 256, 0, st>>>(a);
+    else if (p.S < 128 || n > 8192) reduce_kernel<T, OP, 16><<<dim3((unsigned)((n + 15) / 16)), 256, 0, st>>>(a);
+    else reduce_kernel<T, OP, 64><<<dim3((unsigned)((n + 3) / 4)), 256, 0, st>>>(a);
   }
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }

@@ -92,7 +92,8 @@ def check_linear(x, w, b, r, yb, act, beta, train=True):
 
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 7, 3), (5, 1024, 513), (16, 40, 8), (31, 256, 1), (33, 33, 33), (64, 64, 64), (65, 129, 63), (127, 84, 256),
-         (128, 128, 128), (129, 340, 256), (300, 361, 255), (1000, 63, 129), (4099, 256, 3), (8192, 256, 256), (20000, 39, 217), (16500, 1000, 1030), (3000, 2050, 2000)]
+         (128, 128, 128), (129, 340, 256), (300, 361, 255), (1000, 63, 129), (4099, 256, 3), (8192, 256, 256), (20000, 39, 217), (16500, 1000, 1030), (3000, 2050, 2000),
+         (517, 3, 70), (9, 7, 2), (1030, 1, 5), (16, 1, 16), (3, 5, 3), (2, 3, 400), (40, 15, 1), (700, 9, 7)]
 
 
 @pytest.mark.parametrize("dtype", DT, ids=IDS)
