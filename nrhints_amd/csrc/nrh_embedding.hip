@@ -22,7 +22,7 @@ namespace nrhemb {
 typedef long long ll;
 typedef unsigned long long ull;
 constexpr unsigned NONE = 0xffffffffu;
-constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 16, LOW = 255, LOW_TOKENS = 512;
+constexpr int TILE = 1024, SMALL = 2048, FOLD = 64, RUN0 = 32, RUN1 = 16, LOW = 255, LOW_TOKENS = 512, TAIL = 2048, TAIL_GROUPS = 64;
 
 // V elements at any element-aligned address (global memory takes unaligned vector accesses).  A row of d >= V elements is covered by
 // ceil(d / V) vectors, the last one drawn back to end with the row: what two of them share is the same values twice.
@@ -338,6 +338,106 @@ __global__ __launch_bounds__(256) void sum_kernel(const Level a) {
   }
 }
 
+// One workgroup's sorted entries: groups of `width` lanes (group g, lane l) walk equal shares beg .. end of them, BATCH loads at a time.  A
+// run that ends inside a share is done; the first and the last run of a share meet their neighbours' in LDS (edge: [group][first |
+// last][lane][V], edge_key), where the share in which a run starts adds up the rest.  key(e): the row of entry e or NONE; load(e, x): its
+// values in this lane's columns; finish(row, sums).  Every thread of the workgroup calls it; `on`: the lane has columns (lane 0 of a
+// group does if any does).
+template <int V, int BATCH, typename KEY, typename LOAD, typename FINISH>
+__device__ __forceinline__ void add_shares(int g, int groups, int l, int width, int beg, int end, bool on, float* edge, unsigned* edge_key,
+                                           const KEY& key, const LOAD& load, const FINISH& finish) {
+  float acc[V];
+#pragma unroll
+  for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+  auto keep = [&](int slot, unsigned k) {
+    if (l == 0) edge_key[slot] = k;
+#pragma unroll
+    for (int q = 0; q < V; ++q) edge[(slot * width + l) * V + q] = acc[q];
+  };
+  if (on) {
+    unsigned cur = NONE;
+    bool head = true;
+    for (int e = beg; e < end; e += BATCH) {
+      unsigned k[BATCH];
+      float x[BATCH][V];
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        k[b] = e + b < end ? key(e + b) : NONE;
+        if (e + b < end) load(e + b, x[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (k[b] == NONE) continue;
+        if (k[b] != cur) {
+          if (cur != NONE) {
+            if (head) keep(2 * g, cur);
+            else finish(cur, acc);
+            head = false;
+          }
+          cur = k[b];
+#pragma unroll
+          for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < V; ++q) acc[q] += x[b][q];
+      }
+    }
+    if (head) {
+      keep(2 * g, cur);
+      if (l == 0) edge_key[2 * g + 1] = NONE;
+    } else {
+      keep(2 * g + 1, cur);
+    }
+  }
+  __syncthreads();
+  if (!on) return;
+  for (int slot = 2 * g; slot < 2 * g + 2; ++slot) {
+    const unsigned k = edge_key[slot];
+    bool starts = k != NONE;
+    if (starts) {                                        // ... unless the entry before it is of the same row
+      int s = slot - 1;
+      while (s >= 0 && edge_key[s] == NONE) --s;
+      starts = s < 0 || edge_key[s] != k;
+    }
+    if (!starts) continue;
+#pragma unroll
+    for (int q = 0; q < V; ++q) acc[q] = edge[(slot * width + l) * V + q];
+    for (int s = slot + 1; s < 2 * groups; ++s) {
+      const unsigned ks = edge_key[s];
+      if (ks == NONE) continue;
+      if (ks != k) break;
+#pragma unroll
+      for (int q = 0; q < V; ++q) acc[q] += edge[(s * width + l) * V + q];
+    }
+    finish(k, acc);
+  }
+}
+
+// The last level: at most TAIL entries, 8 vectors of the rows per workgroup.  (Levels of RUN1 down to one run instead: 5 us each.)
+template <typename T, int V>
+__global__ __launch_bounds__(512) void tail_kernel(const Level a) {
+  typedef typename Vec<T, V>::type VT;
+  typedef typename Vec<float, V>::type FT;
+  __shared__ float edge[2 * 512 * V];
+  __shared__ unsigned edge_key[2 * TAIL_GROUPS];
+  const int g = threadIdx.x / a.width, l = threadIdx.x % a.width, c = blockIdx.y * a.width + l;
+  const bool on = g < TAIL_GROUPS && c < a.cols;
+  const ll col = column<V>(c < a.cols ? c : 0, a.d);
+  const int share = ((int)a.n + TAIL_GROUPS - 1) / TAIL_GROUPS, beg = g * share, end = beg + share < a.n ? beg + share : (int)a.n;
+  auto load = [&](int e, float* x) {
+    const FT y = *(const FT*)((const float*)a.rows + (ll)e * a.ldr + col);
+#pragma unroll
+    for (int q = 0; q < V; ++q) x[q] = at<float, V>(y, q);
+  };
+  auto finish = [&](unsigned row, const float* acc) {
+    VT y;
+#pragma unroll
+    for (int q = 0; q < V; ++q) put<T, V>(y, q, a.scale * acc[q]);
+    *(VT*)((T*)a.out + (ll)row * a.ldo + col) = y;
+  };
+  add_shares<V, 8>(g, TAIL_GROUPS, l, a.width, beg, end, on, edge, edge_key, [&](int e) { return a.keys[e]; }, load, finish);
+}
+
 // ---- low tables --------------------------------------------------------------------------------------------------------------
 struct Low {
   const void* index;
@@ -350,14 +450,12 @@ struct Low {
   float* part;                   // [workgroups][v][d]; null: one workgroup, which writes the table
 };
 
-// 512 tokens: counting sort by row in LDS (stable); then groups of lanes walk equal shares of the sorted tokens.  A run that ends inside a
-// share is done; the first and the last run of a share meet their neighbours' in LDS, where the share in which a run starts adds up the rest.
-// blockIdx.y: 64 vectors of the row each.
+// 512 tokens: counting sort by row in LDS (stable), then their sums.  blockIdx.y: 64 vectors of the row each.
 template <typename T, int V>
 __global__ __launch_bounds__(LOW_TOKENS) void low_kernel(const Low a) {
   typedef typename Vec<T, V>::type VT;
   typedef typename Vec<float, V>::type FT;
-  constexpr int WAVES = LOW_TOKENS / 64, BATCH = 8, GROUPS = 32;
+  constexpr int WAVES = LOW_TOKENS / 64, GROUPS = 32;
   __shared__ unsigned cnt[WAVES][256];
   __shared__ unsigned buf[256];
   __shared__ unsigned start[257];
@@ -427,72 +525,15 @@ __global__ __launch_bounds__(LOW_TOKENS) void low_kernel(const Low a) {
       *(VT*)((T*)a.out + row * a.ldo + col) = y;
     }
   };
-  auto keep = [&](int slot, unsigned k, const float* acc) {
-    if (l == 0) edge_key[slot] = k;
+  auto load = [&](int e, float* x) {
+    const VT y = *(const VT*)((const T*)a.rows + (tok0 + order[e]) * a.ldr + col);
 #pragma unroll
-    for (int q = 0; q < V; ++q) edge[(slot * a.width + l) * V + q] = acc[q];
+    for (int q = 0; q < V; ++q) x[q] = at<T, V>(y, q);
   };
-  float acc[V];
-#pragma unroll
-  for (int q = 0; q < V; ++q) acc[q] = 0.0f;
-  if (on) {
-    const int beg = g * share, end = beg + share < named ? beg + share : named;
-    unsigned cur = NONE;
-    bool head = true;
-    for (int e = beg; e < end; e += BATCH) {
-      VT x[BATCH];
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b)
-        if (e + b < end) x[b] = *(const VT*)((const T*)a.rows + (tok0 + order[e + b]) * a.ldr + col);
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b)
-        if (e + b < end) {
-          const unsigned k = sorted[e + b];
-          if (k != cur) {
-            if (cur != NONE) {
-              if (head) keep(2 * g, cur, acc);
-              else finish(cur, acc);
-              head = false;
-            }
-            cur = k;
-#pragma unroll
-            for (int q = 0; q < V; ++q) acc[q] = 0.0f;
-          }
-#pragma unroll
-          for (int q = 0; q < V; ++q) acc[q] += at<T, V>(x[b], q);
-        }
-    }
-    if (head) {
-      keep(2 * g, cur, acc);
-      if (l == 0) edge_key[2 * g + 1] = NONE;
-    } else {
-      keep(2 * g + 1, cur, acc);
-    }
-  } else if (g < groups && l == 0) {
-    edge_key[2 * g] = edge_key[2 * g + 1] = NONE;        // (lane 0 of a group has a column whenever any lane has)
-  }
-  __syncthreads();
-  if (on) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {                          // (two neighbouring slots of one share never hold the same row)
-      const int slot = 2 * g + h;
-      const unsigned k = edge_key[slot];
-      if (k == NONE || (h == 0 && g > 0 && (edge_key[slot - 1] == k || (edge_key[slot - 1] == NONE && edge_key[slot - 2] == k)))) continue;
-#pragma unroll
-      for (int q = 0; q < V; ++q) acc[q] = edge[(slot * a.width + l) * V + q];
-      for (int s = slot + 1; s < 2 * groups; ++s) {
-        const unsigned ks = edge_key[s];
-        if (ks == NONE) continue;
-        if (ks != k) break;
-#pragma unroll
-        for (int q = 0; q < V; ++q) acc[q] += edge[(s * a.width + l) * V + q];
-      }
-      finish(k, acc);
-    }
-  }
+  const int beg = g * share, end = beg + share < named ? beg + share : named;
+  add_shares<V, 8>(g, groups, l, a.width, beg, end, on, edge, edge_key, [&](int e) { return (unsigned)sorted[e]; }, load, finish);
   if (on) {                                              // rows that none of these tokens names
-#pragma unroll
-    for (int q = 0; q < V; ++q) acc[q] = 0.0f;
+    const float acc[V] = {};
     for (int row = g; row < a.v; row += groups)
       if (start[row] == start[row + 1]) finish(row, acc);
   }
@@ -639,25 +680,33 @@ template <typename T, int V> static int backward_as(const Call& c, hipStream_t s
   a.scale = c.scale;
   a.out = c.dst;
   a.ldo = c.ldd;
+  const unsigned wide = (unsigned)((cols + a.width - 1) / a.width);
   ll n = c.n;
-  for (int level = 0; level == 0 || n > 0; ++level) {
+  for (int level = 0;; ++level) {
     const ll g = groups(n, level);
-    const bool last = g <= 1;
     a.n = n;
-    a.run = level == 0 ? RUN0 : RUN1;
     a.keys = level == 0 ? keys[cur] : (const unsigned*)(ws + l.lkeys[(level - 1) & 1]);
     a.perm = perm[cur];
     a.rows = level == 0 ? c.src : (const void*)(ws + l.lrows[(level - 1) & 1]);
     a.ldr = level == 0 ? c.lds : c.d;
-    a.next_keys = last ? nullptr : (unsigned*)(ws + l.lkeys[level & 1]);
+    if (level > 0 && n <= TAIL) {
+      while (a.width > 512 / TAIL_GROUPS) a.width /= 2;
+      tail_kernel<T, V><<<dim3(1, (unsigned)((cols + a.width - 1) / a.width)), 512, 0, st>>>(a);
+      break;
+    }
+    a.run = level == 0 ? RUN0 : RUN1;
+    a.next_keys = g <= 1 ? nullptr : (unsigned*)(ws + l.lkeys[level & 1]);
     a.next_rows = (float*)(ws + l.lrows[level & 1]);
     const int per = 256 / a.width;
     a.sum_blocks = (unsigned)((g + per - 1) / per);
-    const ll clear = (c.v + 63) / 64 < (1 << 20) ? (c.v + 63) / 64 : (1 << 20);      // 16 rows per wave
-    const dim3 grid(a.sum_blocks + (level == 0 ? (unsigned)clear : 0u), (unsigned)((cols + a.width - 1) / a.width));
-    if (level == 0) sum_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
-    else sum_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
-    n = last ? 0 : 2 * g;
+    if (level == 0) {
+      const ll clear = (c.v + 63) / 64 < (1 << 20) ? (c.v + 63) / 64 : (1 << 20);      // 16 rows per wave
+      sum_kernel<T, V, true><<<dim3(a.sum_blocks + (unsigned)clear, wide), 256, 0, st>>>(a);
+    } else {
+      sum_kernel<T, V, false><<<dim3(a.sum_blocks, wide), 256, 0, st>>>(a);
+    }
+    if (g <= 1) break;
+    n = 2 * g;
   }
   return hipGetLastError() == hipSuccess ? 0 : -2;
 }
