@@ -12,9 +12,12 @@
 //     transpose 4 x 16 blocks on the way to the registers.
 // Both are swizzled by 16- or 64-byte groups so that neither the writes nor the reads of a wave meet in a bank.
 // act' is applied on the way to LDS: zbar is never stored.
-//   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' is rounded to the type once, as every operand of a 16-bit
-//     product is; for NONE and RELU it is exact.  act' itself is kept wider than the type (float32 beside float16, float16 beside
-//     bfloat16: 11 bits against 8), so that this one rounding is the only one.
+//   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' has more bits than the type.  For NONE and RELU it is exact.  For
+//     the smooth activations 64 x 64 tiles take it as two parts of the type, the rounded value and the rounded rest (16 bits of
+//     bfloat16, 22 of float16), at two products per pair: they are bound by latency, and it costs little (512 x 256 x 256 bf16: dx 6.5
+//     us against 5.7).  The larger tiles, bound by their products, round it once (16 384 x 1 024 x 1 024: 49 us against 98), as every operand
+//     of a 16-bit product is, which makes the gradients' rms error 1.4 times that of rounding them alone.  act' itself is kept wider
+//     than the type (float32 beside float16, float16 beside bfloat16: 11 bits against 8), so that no other rounding joins these.
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
@@ -39,12 +42,15 @@ typedef short i16x8 __attribute__((ext_vector_type(8)));
 typedef long long ll;
 
 enum Src { ROWS = 0, COLS = 1 };
-enum Deriv { PLAIN = 0, SMOOTH = 1, MASK = 2 };      // A as it is, times act', or kept where act' > 0 (RELU)
+enum Deriv { PLAIN = 0, SMOOTH = 1, MASK = 2, PARTS = 3 };      // A as it is, times act', kept where act' > 0 (RELU), times act' in two parts
 
 template <typename T> struct Ty;                    // planes, LDS element, type act' is kept in
 template <> struct Ty<float> { static constexpr int PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; typedef float D; };
 template <> struct Ty<_Float16> { static constexpr int PLANES = 1; typedef _Float16 L; typedef f16x8 L8; typedef float D; };
 template <> struct Ty<__bf16> { static constexpr int PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; typedef _Float16 D; };
+
+// planes of an operand: the parts it is split into
+template <typename T, int DM> constexpr int planes() { return DM == PARTS ? 2 : Ty<T>::PLANES; }
 
 template <bool C, typename A, typename B> struct Pick { typedef A type; };
 template <typename A, typename B> struct Pick<false, A, B> { typedef B type; };
@@ -252,6 +258,13 @@ template <typename L8, int SRC, int BA, int BK, bool PERM> __device__ __forceinl
   return __builtin_bit_cast(L8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+template <typename L> __device__ __forceinline__ void halves(uint32_t w, float& a, float& b) {      // the two 16-bit floats of a word
+  typedef L L2 __attribute__((ext_vector_type(2)));
+  const L2 t = __builtin_bit_cast(L2, w);
+  a = (float)t[0];
+  b = (float)t[1];
+}
+
 // ---- staging -----------------------------------------------------------------------------------------------------------------
 template <typename T, int DM> struct Factor { typedef typename Ty<T>::D type; };
 template <typename T> struct Factor<T, MASK> { typedef T type; };
@@ -261,7 +274,7 @@ template <typename T> struct Factor<T, MASK> { typedef T type; };
 template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool SINGLE> struct Stage {
   typedef typename Factor<T, DM>::type Q;
   typedef typename Ty<T>::L L;
-  static constexpr int PL = Ty<T>::PLANES, CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
+  static constexpr int PL = planes<T, DM>(), CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
   typedef Tile<SRC, BA, BK> Tl;
   Chunk<T> v[NC];
   Chunk<Q> q[DM != PLAIN ? NC : 1];
@@ -348,15 +361,17 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool S
       if (DM != PLAIN) {
         float f0, f1;
         q_pair(u, e, f0, f1);
-        if (DM == SMOOTH) { x[2 * e] *= f0; x[2 * e + 1] *= f1; }
+        if (DM == SMOOTH || DM == PARTS) { x[2 * e] *= f0; x[2 * e + 1] *= f1; }
         if (DM == MASK) { x[2 * e] = f0 > 0.0f ? x[2 * e] : 0.0f; x[2 * e + 1] = f1 > 0.0f ? x[2 * e + 1] : 0.0f; }
       }
       if (SUMS) { sums[2 * e] += x[2 * e]; sums[2 * e + 1] += x[2 * e + 1]; }
     }
     y[p][e] = pack2<L>(x[2 * e], x[2 * e + 1]);
-    if (PL == 3 && p < 2) {                             // the rest for the next bfloat16
-      x[2 * e] -= __builtin_bit_cast(float, y[p][e] << 16);
-      x[2 * e + 1] -= __builtin_bit_cast(float, y[p][e] & 0xffff0000u);
+    if (p < PL - 1) {                                   // the rest for the next part
+      float h0, h1;
+      halves<L>(y[p][e], h0, h1);
+      x[2 * e] = PL == 3 || fabsf(h0) < __builtin_huge_valf() ? x[2 * e] - h0 : 0.0f;      // (PL 3: NaN, see below)
+      x[2 * e + 1] = PL == 3 || fabsf(h1) < __builtin_huge_valf() ? x[2 * e + 1] - h1 : 0.0f;
     }
     if (e == 3) *(V*)(dst + p * Tl::BYTES) = V{y[p][0], y[p][1], y[p][2], y[p][3]};
   }
@@ -481,20 +496,20 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
 template <int N> struct Const { constexpr operator int() const { return N; } };
 
 // ---- the tile kernel ---------------------------------------------------------------------------------------------------------
-template <typename T, int OP, int WI, int WJ, int NI, int NJ, int BK> struct Shape {
-  static constexpr int PL = Ty<T>::PLANES, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
-  static constexpr int BUF = PL * (BI + BJ) * BK * 2;                               // one step
+template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK> struct Shape {
+  static constexpr int PI = planes<T, DM>(), PJ = planes<T, PLAIN>(), BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
+  static constexpr int BUF = (PI * BI + PJ * BJ) * BK * 2;                               // one step
   static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
-  static constexpr int EXACT = PL == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
+  static constexpr int EXACT = PJ == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
   static constexpr int SUMS = OP == BACK_WEIGHT ? NT * 8 * 4 : 0;
   static constexpr int m1 = 2 * BUF > EPI ? 2 * BUF : EPI, m2 = EXACT > SUMS ? EXACT : SUMS, LDS = m1 > m2 ? m1 : m2;
 };
 
 template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK, int OCC, bool SINGLE>
 __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
-  typedef Shape<T, OP, WI, WJ, NI, NJ, BK> Sh;
+  typedef Shape<T, OP, DM, WI, WJ, NI, NJ, BK> Sh;
   constexpr int SI = OP == BACK_WEIGHT ? COLS : ROWS, SJ = OP == FORWARD ? ROWS : COLS;
-  constexpr int PL = Sh::PL, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
+  constexpr int PI = Sh::PI, PJ = Sh::PJ, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
   typedef typename Ty<T>::L8 L8;
   typedef Stage<T, SI, DM, false, BI, BK, NT, SINGLE> StI;
   typedef Stage<T, SJ, PLAIN, true, BJ, BK, NT, SINGLE> StJ;
@@ -525,27 +540,29 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
   auto piece = [&](int q, int buf) {
     char* b = lds + buf * Sh::BUF;
     if (q < StI::PIECES) si.template piece<OP == BACK_WEIGHT>(q, px, py, b, bs, tid);
-    else sj.template piece<false>(q - StI::PIECES, px, py, b + PL * StI::Tl::BYTES, nullptr, tid);
+    else sj.template piece<false>(q - StI::PIECES, px, py, b + PI * StI::Tl::BYTES, nullptr, tid);
   };
 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
   f32x16 acc[NI][NJ] = {};
-  constexpr int READS = (NI + NJ) * PL, MF = NI * NJ * (PL == 3 ? 6 : 1);      // per 16 values of the reduction
+  constexpr int READS = NI * PI + NJ * PJ, MF = NI * NJ * (PJ == 3 ? 6 : PI);      // per 16 values of the reduction
   constexpr int PUT0 = KK > 2 ? KK - 3 : 0, PUTS = KK - 1 - PUT0;              // the sixteens beside which the next step goes to LDS
   static_assert(KK >= 2, "");
-  struct Operands { L8 i[NI][PL], j[NJ][PL]; };
+  struct Operands { L8 i[NI][PI], j[NJ][PJ]; };
   Operands f[2];
   auto read = [&](Operands& o, int kk, int q, int buf) {
     const char* bi = lds + buf * Sh::BUF;
-    const char* bj = bi + PL * StI::Tl::BYTES;
-    const int p = q / (NI + NJ), b = q % (NI + NJ);
+    const char* bj = bi + PI * StI::Tl::BYTES;
+    // the plane that both have first, then the others
+    const int both = PI < PJ ? PI : PJ, p = q < both * (NI + NJ) ? q / (NI + NJ) : both + (q - both * (NI + NJ)) / NI;
+    const int b = q < both * (NI + NJ) ? q % (NI + NJ) : (q - both * (NI + NJ)) % NI;
     if (b < NI) o.i[b % NI][p] = fragment<L8, SI, BI, BK, false>(bi + p * StI::Tl::BYTES, wi * NI + b, kk, lane);
-    else o.j[(b - NI) % NJ][p] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b - NI, kk, lane);
+    else o.j[(b - NI) % NJ][p % PJ] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b - NI, kk, lane);
   };
   auto product = [&](const Operands& o, int q) {       // the small products first
-    constexpr int PI[6] = {2, 0, 1, 0, 1, 0}, PJ[6] = {0, 2, 1, 1, 0, 0};
+    constexpr int QI[6] = {2, 0, 1, 0, 1, 0}, QJ[6] = {0, 2, 1, 1, 0, 0};
     const int t = q / (NI * NJ), x = q % (NI * NJ) / NJ, y = q % NJ;
-    acc[x][y] = mfma(o.j[y][PL == 3 ? PJ[t] : 0], o.i[x][PL == 3 ? PI[t] : 0], acc[x][y]);
+    acc[x][y] = mfma(o.j[y][PJ == 3 ? QJ[t] : 0], o.i[x][PJ == 3 ? QI[t] : PI - 1 - t], acc[x][y]);
   };
   // The kk-th 16 values of a step, and between their MFMAs - in this order, a few instructions after each - the reads of the next
   // sixteen's operands (READ; the last one reads the next step's first, from the other buffer) and pieces of the next step's way to LDS.
@@ -591,7 +608,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     sixteen(Const<KK - 1>(), No(), No(), buf);
   }
 
-  if (PL == 3) {
+  if (PJ == 3) {
     int bad = 0;
 #pragma unroll
     for (int x = 0; x < NI; ++x)
@@ -826,9 +843,10 @@ static Size size_of(int dtype, int v) {
 // S > 1 splits' parts: JOIN + I J (S PART + LAST).  Fitted (rms 12 %) to 600 timings of 20 shapes from 64 x 1 024 x 1 024 to
 // 400 000 x 256 x 256, every variant at 1 to 256 splits; the choice by it is on average 2 % above the best of each.
 struct Cost { float start, alone, each, tile; };
-static Cost cost_of(int dtype, bool act_bar, int v) {
+static Cost cost_of(int dtype, bool act_bar, bool parts, int v) {
   if (v == TINY) return {4.0f, 0.036f, 0.006f, 0.30f};
   if (dtype == F32) return v <= SMALL ? Cost{4.0f, 0.0234f, 0.0156f, 0.31f} : Cost{7.9f, 0.0388f, 0.0644f, 7.6f};
+  if (v <= SMALL && parts) return {3.95f, 0.0141f, 0.0088f, 0.28f};
   if (v <= SMALL) return act_bar ? Cost{3.6f, 0.0109f, 0.0065f, 0.18f} : Cost{3.4f, 0.0092f, 0.0042f, 0.46f};
   if (v == MIDDLE) return act_bar ? Cost{5.6f, 0.0121f, 0.0164f, 0.60f} : Cost{5.75f, 0.0011f, 0.0121f, 0.89f};
   return act_bar ? Cost{8.3f, 0.0093f, 0.0343f, 7.2f} : Cost{8.2f, 0.0040f, 0.0295f, 7.1f};
@@ -855,7 +873,7 @@ static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
   for (int v = tiny ? TINY : SMALL; v <= (tiny ? TINY : LARGE); ++v) {
     if (v == MIDDLE && dtype == F32) continue;
     const Size z = size_of(dtype, v);
-    const Cost c = cost_of(dtype, act_bar, v);
+    const Cost c = cost_of(dtype, act_bar, act_bar && act != RELU, v);
     const ll TI = (I + z.i - 1) / z.i, TJ = (J + z.j - 1) / z.j;
     for (int s = 1; s <= MOST && s <= steps; s = s < 4 ? s + 1 : s + (s & (s - 1) ? s / 3 : s / 2)) {      // 1 2 3 4 6 8 12 16 ..
       const ll chunk = (steps + s - 1) / s, S = (steps + chunk - 1) / chunk, n = TI * TJ * S;
@@ -886,7 +904,7 @@ long long workspace_bytes(int op, int dtype, int act, long long m, long long n, 
 
 // more than 64 KB of LDS has to be asked for, once per kernel and device (idempotent: no lock)
 template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK, int OCC, bool SINGLE = false> static int start(const Args& a, unsigned grid, hipStream_t st) {
-  typedef Shape<T, OP, WI, WJ, NI, NJ, BK> Sh;
+  typedef Shape<T, OP, DM, WI, WJ, NI, NJ, BK> Sh;
   static bool ready[64];
   int dev = -1;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return -2;
@@ -900,12 +918,13 @@ template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK, in
 }
 
 template <typename T, int OP, int DM> static int start_tile(const Args& a, int variant, unsigned grid, hipStream_t st) {
-  if (variant == TINY) return start<T, OP, DM, 2, 2, 1, 1, 32, 2, true>(a, grid, st);
+  constexpr int DS = sizeof(T) == 2 && DM == SMOOTH ? PARTS : DM;
+  if (variant == TINY) return start<T, OP, DS, 2, 2, 1, 1, 32, 2, true>(a, grid, st);
   if constexpr (sizeof(T) == 4) {
     if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 32, 2>(a, grid, st);
     return start<T, OP, DM, 4, 2, 2, 2, 32, 2>(a, grid, st);
   } else {
-    if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 64, 2>(a, grid, st);
+    if (variant == SMALL) return start<T, OP, DS, 2, 2, 1, 1, 64, 2>(a, grid, st);
     if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, DM == PLAIN ? 64 : 32, 2>(a, grid, st);      // (act' takes registers)
     return start<T, OP, DM, 2, 2, 2, 2, 64, 2>(a, grid, st);
   }
