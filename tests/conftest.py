@@ -14,7 +14,7 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
 
 
-# Eight processes that each render a 640 000-ray frame and train on ONE GPU print nothing until they are done: 24 s on the boxes this was
+# Eight processes that each render a 640 000-ray frame and train on ONE GPU print nothing until they are done: 24 s where it was
 # written on, more than 180 s where the processes time-slice the GPU slowly (the two-rank case: 9 s against 32 s, with the same kernels).
 # A run that is silent for that long cannot be told from a hung one, so the case is not run.
 OFF = {"test_bench_rehearsal_on_one_gpu[8-weak-0]": "silent for minutes where eight processes share one GPU slowly; indistinguishable from a hang"}

@@ -499,3 +499,40 @@ def test_a_capture_beside_a_live_eager_graph_is_refused():
         gr.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(want, grads))
+
+
+@pytest.mark.parametrize("dtype", DT[1:], ids=IDS[1:])
+@pytest.mark.parametrize("act", ["softplus", "sigmoid", "silu", "gelu"])
+def test_small_gradients_are_rounded_once(dtype, act):
+    """Small 16-bit products take ybar act' in two parts (the type's bits twice: 2^-16 of bfloat16 at least), so what a gradient is off by is
+    its own rounding, that of the kept act' (beside bfloat16: float16) and float32's."""
+    m, k, n, beta = 200, 96, 130, 1.0
+    x, w, b, _, yb = operands(m, k, n, dtype, act, 77)
+    y, dact = ops.linear_train_forward(x, w, b, activation=act, beta=beta)
+    xb, wb, _ = ops.linear_backward(yb, x, w, dact, activation=act)
+    X, W, YB = x.double(), w.double(), yb.double()
+    z = (X @ W.t() + b.double()).requires_grad_(True)
+    d = torch.autograd.grad(act64(z, act, beta).sum(), z)[0]
+    z = z.detach()
+    ez = (k + 8) * U32 * (X.abs() @ W.abs().t() + b.double().abs())
+    ed = CURVATURE[act] * ez + 16 * U32 * (1.0 + (z.abs() if act in ("silu", "gelu") else 0.0))
+    kept = ut(torch.float16) * d.abs() + 2.0 ** -25 if dtype == torch.bfloat16 else 0.0
+    zb = YB * d
+    ezb = YB.abs() * (ed + kept) + 2.0 ** -16 * zb.abs() + (2.0 ** -25 if dtype == torch.float16 else 0.0)
+    for got, want, err in ((xb, zb @ W, ezb @ W.abs() + (2 * n + 8) * U32 * (zb.abs() @ W.abs())),
+                           (wb, zb.t() @ X, ezb.t() @ X.abs() + (2 * m + 8) * U32 * (zb.abs().t() @ X.abs()))):
+        bound = err + 1.01 * ut(dtype) * want.abs() + tiny(dtype)
+        assert bool(((got.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("ld", [3950000, 4200000])
+def test_linear_offsets_past_32_bits(ld):
+    """Rows so far apart that the last ones lie beyond 2^32 elements, on either side of the 2^22 up to which lanes keep 32-bit offsets."""
+    m, k, n = 1100, 72, 40
+    g = gen(5)
+    store = torch.empty((m, ld), dtype=torch.float16, device="cuda")
+    assert store.stride(0) * (m - 1) > 2 ** 32
+    x = store[:, 5:5 + k]
+    x.copy_(torch.randn(m, k, generator=g, device="cuda"))
+    w = (torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)).half()
+    check_linear(x, w, None, None, torch.randn(m, n, generator=g, device="cuda").half(), "silu", 1.0)
