@@ -27,9 +27,9 @@ def _same_side_of_capture(*tensors) -> None:
     """A parameter's gradient is accumulated on the stream its graph was first recorded on.  If an eager graph of the parameter is still
     alive, a backward pass captured now would accumulate on the eager stream and end the process: refuse it here, while an exception
     still can."""
-    capturing = torch.cuda.is_current_stream_capturing()
     for t in tensors:
-        if t is not None and t.requires_grad and t.is_leaf:
+        if t is not None and t.is_cuda and t.requires_grad and t.is_leaf:
+            capturing = torch.cuda.is_current_stream_capturing()
             meta = get_gradient_edge(t).node.metadata
             if not capturing:
                 meta[_EAGER] = True
