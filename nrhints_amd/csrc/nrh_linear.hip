@@ -845,7 +845,7 @@ static Size size_of(int dtype, int v) {
 }
 
 // What a launch takes, in microseconds, with w tiles per CU that each reduce L values: start + L max(alone, w each) + (w - 1) tile; and
-// S > 1 splits' parts: JOIN + I J (S PART + LAST).  Fitted (rms 12 %) to 600 timings of 20 shapes from 64 x 1 024 x 1 024 to
+// S > 1 splits' parts: JOIN + I J (S PART + LAST).  Fitted (rms 12 %) to 2 034 timings of 20 shapes from 64 x 1 024 x 1 024 to
 // 400 000 x 256 x 256, every variant at 1 to 256 splits; the choice by it is on average 2 % above the best of each.
 struct Cost { float start, alone, each, tile; };
 static Cost cost_of(int dtype, bool act_bar, bool parts, int v) {
