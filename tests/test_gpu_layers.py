@@ -93,7 +93,7 @@ def check_linear(x, w, b, r, yb, act, beta, train=True):
 
 SIZES = [(1, 1, 1), (1, 256, 256), (2, 7, 3), (5, 1024, 513), (16, 40, 8), (31, 256, 1), (33, 33, 33), (64, 64, 64), (65, 129, 63), (127, 84, 256),
          (128, 128, 128), (129, 340, 256), (300, 361, 255), (1000, 63, 129), (4099, 256, 3), (8192, 256, 256), (20000, 39, 217), (16500, 1000, 1030), (3000, 2050, 2000),
-         (517, 3, 70), (9, 7, 2), (1030, 1, 5), (16, 1, 16), (3, 5, 3), (2, 3, 400), (40, 15, 1), (700, 9, 7)]
+         (517, 3, 70), (9, 7, 2), (1030, 1, 5), (16, 1, 16), (3, 5, 3), (2, 3, 400), (40, 15, 1), (700, 9, 7), (9, 8, 8), (17, 16, 1), (70000, 3, 2), (2, 7001, 3), (3, 2, 7001)]
 
 
 @pytest.mark.parametrize("dtype", DT, ids=IDS)
@@ -536,3 +536,55 @@ def test_linear_offsets_past_32_bits(ld):
     x.copy_(torch.randn(m, k, generator=g, device="cuda"))
     w = (torch.randn(n, k, generator=g, device="cuda") / math.sqrt(k)).half()
     check_linear(x, w, None, None, torch.randn(m, n, generator=g, device="cuda").half(), "silu", 1.0)
+
+
+def test_calls_at_once_and_two_graphs_of_one_pool():
+    """The same bits from three streams at once and from two graphs that share a memory pool, replayed between eager work."""
+    g = gen(12)
+    x, yb = torch.randn(4096, 300, generator=g, device="cuda").half(), torch.randn(4096, 500, generator=g, device="cuda").half()
+    w = (torch.randn(500, 300, generator=g, device="cuda") / 17).half()
+    index, rows = torch.randint(0, 700, (20000,), generator=g, device="cuda"), torch.randn(20000, 37, generator=g, device="cuda")
+    _, dact = ops.linear_train_forward(x, w, activation="gelu")
+
+    def work():
+        return (*ops.linear_backward(yb, x, w, dact, activation="gelu", want_bias=True), ops.embedding_backward(rows, index, 700))
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(4):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for o in got for a, b in zip(o, want))
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    with torch.cuda.graph(graphs[0]):
+        work()
+    with torch.cuda.graph(graphs[1], pool=graphs[0].pool()):
+        last = work()
+    for _ in range(4):
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(last, want))
+        ops.linear(x, w)
+        torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("v,d,n", [(1, 1, 1), (255, 8, 513), (256, 8, 1024), (256, 9, 1025), (5, 1 << 20, 3), (300, 3, 2049), (300, 100000, 40),
+                                   (70000, 5, 65537), (2, 4, 0), (10, 7, 12), (60000, 20, 8193)])
+def test_embedding_gradient_at_its_limits(v, d, n):
+    """Either side of each rule (255 rows, 1 024 tokens, rows of 16 bytes, 64 tiles), against sums in float64: a row's sum of t terms is off
+    by at most t u32 sum |rows| and one rounding."""
+    for dtype in (torch.float32, torch.bfloat16):
+        g = gen(v + d + n)
+        rows, index = torch.randn(n, d, generator=g, device="cuda").to(dtype), torch.randint(-1, v + 1, (n,), generator=g, device="cuda")
+        got = ops.embedding_backward(rows, index, v)
+        ok = (index >= 0) & (index < v)
+        want, size, terms = (torch.zeros(v, d, dtype=torch.float64, device="cuda") for _ in range(3))
+        want.index_add_(0, index[ok], rows.double()[ok])
+        size.index_add_(0, index[ok], rows.double()[ok].abs())
+        terms.index_add_(0, index[ok], torch.ones_like(rows, dtype=torch.float64)[ok])
+        assert bool(((got.double() - want).abs() <= (terms + 1) * U32 * size + 1.01 * ut(dtype) * want.abs() + tiny(dtype)).all())
