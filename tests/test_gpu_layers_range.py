@@ -1,0 +1,88 @@
+"""The layer operators away from values of size one: saturated activations, small and large gradients, infinities, subnormal numbers.
+
+u32 = 2^-24.  Arguments are one product with 1, so they are exact; act' is then off by at most 24 u32 of its value: 2 for the exponential,
+6 for the complementary error function, 1 for every other step of at most ten, and (softplus) 4 for log or division by beta - never by an
+absolute amount.  ybar act' as an operand of a 16-bit product: two bfloat16 parts leave out at most 2^-17 of it and the low parts' product
+2^-18 (2^-16 together); bfloat16's larger tiles round it once, 2^-9.  Float32 sums of R terms add (R + 8) u32 of the sum of magnitudes, twice
+that in two parts; an output is rounded once (float16: half a subnormal step, 2^-25, at least)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from nrhints_amd import layers, ops  # noqa: E402
+
+U32 = 2.0 ** -24
+DT = [torch.float32, torch.float16, torch.bfloat16]
+IDS = ["f32", "f16", "bf16"]
+LEFT_OUT = {torch.float32: 0.0, torch.float16: 2.0 ** -16, torch.bfloat16: 1.01 * 2.0 ** -9}
+LOWEST = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def slope(z, act, beta):
+    """act'(z) in float64 without the cancellation of 1 + erf or 1 - sigmoid in the tails."""
+    s = lambda t: torch.where(t > 0, 1 / (1 + torch.exp(-t.abs())), torch.exp(-t.abs()) / (1 + torch.exp(-t.abs())))
+    if act == "sigmoid":
+        return s(z) * s(-z)
+    if act == "softplus":
+        return s(beta * z)
+    if act == "silu":
+        return s(z) * (1 + z * s(-z))
+    return 0.5 * torch.special.erfc(-z / math.sqrt(2)) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+
+
+def value(z, act, beta):
+    if act == "sigmoid":
+        return torch.where(z > 0, 1 / (1 + torch.exp(-z.abs())), torch.exp(-z.abs()) / (1 + torch.exp(-z.abs())))
+    if act == "softplus":
+        return z.clamp(min=0) + torch.log1p(torch.exp(-(beta * z).abs())) / beta
+    return z * (value(z, "sigmoid", 1.0) if act == "silu" else 0.5 * torch.special.erfc(-z / math.sqrt(2)))
+
+
+def within(name, got, want, bound):
+    assert got.shape == want.shape
+    err = (got.double() - want).abs()
+    assert bool((err <= bound).all()), (name, float((err / bound).max()))
+
+
+def check_gradients(xb, wb, bb, zb, x, w, dtype):
+    """The three gradients against float64 ones of zb (float64, off by 24 u32 and what the type leaves out of it), purely relative."""
+    X, W, (m, n), ut = x.double(), w.double(), zb.shape, torch.finfo(dtype).eps / 2
+    size, rel = zb.abs(), 24 * U32 + LEFT_OUT[dtype]
+    for name, got, want, sums, r in (("x", xb, zb @ W, size @ W.abs(), n), ("w", wb, zb.t() @ X, size.t() @ X.abs(), m)):
+        within(name, got, want, (rel + (2 * r + 8) * U32) * sums + 1.01 * ut * want.abs() + LOWEST[dtype])
+    if bb is not None:
+        within("b", bb, zb.sum(0), (25 + m + 8) * U32 * size.sum(0) + 1.01 * ut * zb.sum(0).abs() + LOWEST[dtype])
+
+
+def column_of_arguments(m, n, lo, hi, dtype, seed):
+    """x [m, 24], w [n, 24] with z = x w^T = a number of the type in lo .. hi for every row: column 0 holds it beside a weight of 1, the next
+    8 meet zero weights (their weight gradients are sums over rows), the last 15 are zero beside random weights."""
+    g = gen(seed)
+    z = (lo + (hi - lo) * torch.rand(m, generator=g, device="cuda")).to(dtype)
+    x, w = torch.zeros(m, 24, dtype=dtype, device="cuda"), torch.zeros(n, 24, dtype=dtype, device="cuda")
+    x[:, 0], w[:, 0] = z, 1.0
+    x[:, 1:9] = torch.rand(m, 8, generator=g, device="cuda").to(dtype) + 0.5
+    w[:, 9:] = torch.rand(n, 15, generator=g, device="cuda").to(dtype) + 0.5
+    return z, x, w
+
+
+TAILS = [("sigmoid", 1.0, -20.0, -10.0), ("softplus", 1.0, -20.0, -10.0), ("softplus", 100.0, -0.8, -0.1), ("silu", 1.0, -20.0, -10.0), ("gelu", 1.0, -11.0, -5.0)]
+
+
+@pytest.mark.parametrize("act,beta,lo,hi", TAILS + [("gelu", 1.0, -5.0, 8.0), ("softplus", 100.0, -0.1, 0.5)])
+def test_float32_values_in_the_tails(act, beta, lo, hi):
+    """y to 24 u32 of its own value (not of the argument's), on one row and on tiles."""
+    for m in (4, 3000):
+        z, x, w = column_of_arguments(m, 40, lo, hi, torch.float32, 8)
+        y, dact = ops.linear_train_forward(x, w, None, None, act, beta)
+        z = z.double()[:, None].expand(m, 40)
+        within("y", y, value(z, act, beta), 24 * U32 * value(z, act, beta).abs())
+        if hi < 0:
+            within("act'", dact, slope(z, act, beta), 24 * U32 * slope(z, act, beta).abs())
