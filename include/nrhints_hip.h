@@ -646,8 +646,8 @@ int nrh_sdf32_tables(const float* const* sdf_bias, const int* rows, const float*
  *
  * nrh_linear_forward   y [m,n] = act(x [m,k] w [n,k]^T + bias [n]) + residual [m,n]; bias, residual may be null.  activation: 0 none,
  *   1 ReLU, 2 softplus log(1 + exp(beta z)) / beta, 3 sigmoid, 4 SiLU z sigmoid(z), 5 GELU (erf form).  dact [m,n] (contiguous, may be
- *   null): act'(z), what the backward entries need - float32 beside float32 and float16 tensors, float16 beside bfloat16 (wider than
- *   the type: the rounding of ybar act' then is the only one); for ReLU 1 or 0 in the tensors' type.  float32 products are six bfloat16 MFMAs over three-way split operands (float32
+ *   null): act'(z), what the backward entries need - float32 beside every type (a saturated unit's act' is far below float16's range and
+ *   its gradient need not be); for ReLU 1 or 0 in the tensors' type.  float32 products are six bfloat16 MFMAs over three-way split operands (float32
  *   accuracy at any magnitude; tiles with infinities or NaN are computed with float32 MFMAs).
  * nrh_linear_backward_data     xbar [m,k] = (ybar dact) w
  * nrh_linear_backward_weight   wbar [n,k] = (ybar dact)^T x, bias_bar [n] = column sums of ybar dact (may be null); m = 0 gives zeros.

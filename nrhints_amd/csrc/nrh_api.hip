@@ -1850,9 +1850,9 @@ static int layer_result(int rc, const char* who) {
   return NRH_OK;
 }
 
-// act' is kept in float32 beside float16, in float16 beside bfloat16, and as a mask of the tensors' type for ReLU
+// act' is kept in float32, and as a mask of the tensors' type for ReLU
 static bool dact_off_element(const void* p, int dtype, int act) {
-  return ((uintptr_t)p % (dtype == 0 || (dtype == 1 && act != nrhlin::RELU) ? 4 : 2)) != 0;
+  return ((uintptr_t)p % (dtype == 0 || act != nrhlin::RELU ? 4 : 2)) != 0;
 }
 
 static bool off_element(const void* p, int dtype) { return ((uintptr_t)p % (dtype == 0 ? 4 : 2)) != 0; }

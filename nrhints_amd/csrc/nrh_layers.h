@@ -25,8 +25,8 @@ struct Call {
   long long ldr;
   const void* ybar;         // BACK_*
   long long ldyb;
-  const void* dact;         // BACK_*: act'(z) in float32 (F32, F16) or float16 (BF16), or - RELU - anything of the tensors' type that
-                            // is positive exactly where z is; null: activation NONE
+  const void* dact;         // BACK_*: act'(z) in float32, or - RELU - anything of the tensors' type that is positive exactly where z
+                            // is; null: activation NONE
   long long ldd;
   void* out;                // y | xbar | wbar, rows of ldo elements
   long long ldo;

@@ -16,8 +16,8 @@
 //     the smooth activations 64 x 64 tiles take it as two parts of the type, the rounded value and the rounded rest (16 bits of
 //     bfloat16, 22 of float16), at two products per pair: they are bound by latency, and it costs little (512 x 256 x 256 bf16: dx 6.5
 //     us against 5.7).  The larger tiles, bound by their products, round it once (16 384 x 1 024 x 1 024: 49 us against 98), as every operand
-//     of a 16-bit product is, which makes the gradients' rms error 1.4 times that of rounding them alone.  act' itself is kept wider
-//     than the type (float32 beside float16, float16 beside bfloat16: 11 bits against 8), so that no other rounding joins these.
+//     of a 16-bit product is, which makes the gradients' rms error 1.4 times that of rounding them alone.  act' itself is kept in
+//     float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20) keeps all its bits.
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
@@ -48,10 +48,10 @@ typedef long long ll;
 enum Src { ROWS = 0, COLS = 1 };
 enum Deriv { PLAIN = 0, SMOOTH = 1, MASK = 2, PARTS = 3 };      // A as it is, times act', kept where act' > 0 (RELU), times act' in two parts
 
-template <typename T> struct Ty;                    // planes, LDS element, type act' is kept in
-template <> struct Ty<float> { static constexpr int PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; typedef float D; };
-template <> struct Ty<_Float16> { static constexpr int PLANES = 1; typedef _Float16 L; typedef f16x8 L8; typedef float D; };
-template <> struct Ty<__bf16> { static constexpr int PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; typedef _Float16 D; };
+template <typename T> struct Ty;                    // planes, LDS element
+template <> struct Ty<float> { static constexpr int PLANES = 3; typedef __bf16 L; typedef bf16x8 L8; };
+template <> struct Ty<_Float16> { static constexpr int PLANES = 1; typedef _Float16 L; typedef f16x8 L8; };
+template <> struct Ty<__bf16> { static constexpr int PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; };
 
 // planes of an operand: the parts it is split into
 template <typename T, int DM> constexpr int planes() { return DM == PARTS ? 2 : Ty<T>::PLANES; }
@@ -273,7 +273,7 @@ template <typename L> __device__ __forceinline__ void halves(uint32_t w, float& 
 }
 
 // ---- staging -----------------------------------------------------------------------------------------------------------------
-template <typename T, int DM> struct Factor { typedef typename Ty<T>::D type; };
+template <typename T, int DM> struct Factor { typedef float type; };      // act' in memory
 template <typename T> struct Factor<T, MASK> { typedef T type; };
 
 // One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: a tensor may hold fewer than
@@ -397,7 +397,7 @@ __device__ __forceinline__ float finish(const Args& a, ll i, ll j, float z, floa
 
 template <typename T> __device__ __forceinline__ void keep(const Args& a, ll e, float d) {
   if (a.act == RELU) ((T*)a.dact)[e] = (T)d;
-  else ((typename Ty<T>::D*)a.dact)[e] = (typename Ty<T>::D)d;
+  else ((float*)a.dact)[e] = d;
 }
 
 // N floats -> N elements of type X at any element-aligned address, 16 bytes per store
@@ -491,7 +491,7 @@ __device__ __forceinline__ void emit(const Args& a, void* out, ll ldo, const flo
           }
           if (a.dact && MODE != NONE) {
             if constexpr (MODE == RELU) put<T, C>((T*)a.dact + i * a.J + j, d, left);
-            else put<typename Ty<T>::D, C>((typename Ty<T>::D*)a.dact + i * a.J + j, d, left);
+            else put<float, C>((float*)a.dact + i * a.J + j, d, left);
           }
         }
         put<T, C>((T*)out + i * ldo + j, z, left);

@@ -299,8 +299,6 @@ def color_composite(color, weights, wsum, background=None, inside=None, grad=Non
 ACTIVATIONS = ("none", "relu", "softplus", "sigmoid", "silu", "gelu")
 _ACT = {name: code for code, name in enumerate(ACTIVATIONS)}
 _DTYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-#: what act' is kept in between forward and backward (ReLU: a mask of the tensors' own type)
-_DACT = {torch.float32: torch.float32, torch.float16: torch.float32, torch.bfloat16: torch.float16}
 
 
 def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str, dtype=None):
@@ -392,7 +390,7 @@ def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
     y = x.new_empty(shape)
     dact = None
     if want_dact and code != 0 and not (code == 1 and residual is None):
-        dact = x.new_empty(shape, dtype=x.dtype if code == 1 else _DACT[x.dtype])
+        dact = x.new_empty(shape, dtype=x.dtype if code == 1 else torch.float32)
     ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 0, dtype, code, m, n, k)
     with _Here(x.device) as stream:
         rc = _lib.load().nrh_linear_forward(dtype, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _vp(b1), _vp(r2), ldr, code, beta, m, n, k,
@@ -415,9 +413,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
 def linear_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                          residual: Optional[torch.Tensor] = None, activation: str = "none",
                          beta: float = 100.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) - float32 beside
-    float32 and float16, float16 beside bfloat16 -, None for "none", a mask for "relu": y itself where there is no residual (do not change
-    y in place before the backward then)."""
+    """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) in float32, None for
+    "none", a mask of x's type for "relu": y itself where there is no residual (do not change y in place before the backward then)."""
     return _linear_forward(x, weight, bias, residual, activation, beta, True)
 
 
@@ -432,7 +429,7 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
     if (dact is None) != (code == 0):
         raise ValueError("linear_backward: dact (from linear_train_forward) is needed exactly when there is an activation")
     (x2, ldx), (w2, ldw), (g2, ldg) = _matrix(x, m, k, x, "x"), _matrix(weight, n, k, x, "weight"), _matrix(y_bar, m, n, x, "y_bar")
-    d2, ldd = (None, 0) if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else _DACT[x.dtype])
+    d2, ldd = (None, 0) if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else torch.float32)
     lib = _lib.load()
     x_bar = x.new_empty(x.shape) if want_x else None
     w_bar = x.new_empty((n, k)) if (want_weight or want_bias) else None

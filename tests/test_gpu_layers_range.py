@@ -61,15 +61,15 @@ def check_gradients(xb, wb, bb, zb, x, w, dtype):
         within("b", bb, zb.sum(0), (25 + m + 8) * U32 * size.sum(0) + 1.01 * ut * zb.sum(0).abs() + LOWEST[dtype])
 
 
-def column_of_arguments(m, n, lo, hi, dtype, seed):
-    """x [m, 24], w [n, 24] with z = x w^T = a number of the type in lo .. hi for every row: column 0 holds it beside a weight of 1, the next
-    8 meet zero weights (their weight gradients are sums over rows), the last 15 are zero beside random weights."""
+def column_of_arguments(m, n, lo, hi, dtype, seed, k=24):
+    """x [m, k], w [n, k] with z = x w^T = a number of the type in lo .. hi for every row: column 0 holds it beside a weight of 1, the next
+    third meets zero weights (their weight gradients are sums over rows), the others are zero beside random weights."""
     g = gen(seed)
     z = (lo + (hi - lo) * torch.rand(m, generator=g, device="cuda")).to(dtype)
-    x, w = torch.zeros(m, 24, dtype=dtype, device="cuda"), torch.zeros(n, 24, dtype=dtype, device="cuda")
+    x, w = torch.zeros(m, k, dtype=dtype, device="cuda"), torch.zeros(n, k, dtype=dtype, device="cuda")
     x[:, 0], w[:, 0] = z, 1.0
-    x[:, 1:9] = torch.rand(m, 8, generator=g, device="cuda").to(dtype) + 0.5
-    w[:, 9:] = torch.rand(n, 15, generator=g, device="cuda").to(dtype) + 0.5
+    x[:, 1:k // 3] = torch.rand(m, k // 3 - 1, generator=g, device="cuda").to(dtype) + 0.5
+    w[:, k // 3:] = torch.rand(n, k - k // 3, generator=g, device="cuda").to(dtype) + 0.5
     return z, x, w
 
 
@@ -86,3 +86,18 @@ def test_float32_values_in_the_tails(act, beta, lo, hi):
         within("y", y, value(z, act, beta), 24 * U32 * value(z, act, beta).abs())
         if hi < 0:
             within("act'", dact, slope(z, act, beta), 24 * U32 * slope(z, act, beta).abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("act,beta,lo,hi", TAILS, ids=[f"{t[0]}{t[1]:g}" for t in TAILS])
+@pytest.mark.parametrize("m,k,n", [(6, 24, 16), (300, 24, 130), (3, 12, 5), (4096, 24, 2048), (16384, 512, 512)])
+def test_gradients_where_an_activation_is_saturated(m, k, n, act, beta, lo, hi, dtype):
+    """Every argument in the tail: act' is far below 2^-24 there, and the gradients of a loss whose ybar makes up for it (1 / y of a
+    logarithm, say) are ordinary numbers, right to their own last bits."""
+    z, x, w = column_of_arguments(m, n, lo, hi, dtype, 3, k)
+    y, dact = ops.linear_train_forward(x, w, None, None, act, beta)
+    d = slope(z.double(), act, beta)[:, None].expand(m, n)
+    big = (1.0 / d.abs()).clamp(max=3e4 if dtype == torch.float16 else 1e30)
+    yb = (big * (0.5 + torch.rand(m, n, generator=gen(4), device="cuda"))).to(dtype)
+    xb, wb, bb = ops.linear_backward(yb, x, w, dact, act)
+    check_gradients(xb, wb, bb, yb.double() * d, x, w, dtype)
