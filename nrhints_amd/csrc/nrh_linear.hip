@@ -21,8 +21,10 @@
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
-//     is scaled.  Infinities, NaN and values that round up to infinity make the parts NaN: a tile whose sums are not all finite is
-//     computed again with v_mfma_f32_32x32x2_f32, so its results are those of float32 arithmetic.
+//     is scaled.
+// Operands in parts: infinities, NaN and values that round up to infinity make the parts NaN, and an infinity on the other side
+// meets parts that are zero or of the other sign.  A tile whose sums are not all finite is computed again with
+// v_mfma_f32_32x32x2_f32, so its results are those of float32 arithmetic.
 // The MFMA's A role is played by the j operand, its rows permuted (column j = 16 h + 4 q + s of a block of 32 is MFMA row
 // 8 q + 4 h + s): a lane then holds 16 consecutive columns of ONE output row.
 // Measured: 16 384 x 1 024 x 1 024 bf16 38 us (0.9 PFLOP/s; a large library product reaches 1.6), 8 192 x 2 048 x 2 048 67 us (1.0);
@@ -377,8 +379,8 @@ template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool S
     if (p < PL - 1) {                                   // the rest for the next part
       float h0, h1;
       halves<L>(y[p][e], h0, h1);
-      x[2 * e] = PL == 3 || fabsf(h0) < __builtin_huge_valf() ? x[2 * e] - h0 : 0.0f;      // (PL 3: NaN, see below)
-      x[2 * e + 1] = PL == 3 || fabsf(h1) < __builtin_huge_valf() ? x[2 * e + 1] - h1 : 0.0f;
+      x[2 * e] -= h0;                                   // (NaN of an infinity: the tile is computed again)
+      x[2 * e + 1] -= h1;
     }
     if (e == 3) *(V*)(dst + p * Tl::BYTES) = V{y[p][0], y[p][1], y[p][2], y[p][3]};
   }
@@ -507,7 +509,7 @@ template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK> st
   static constexpr int PI = planes<T, DM>(), PJ = planes<T, PLAIN>(), BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
   static constexpr int BUF = (PI * BI + PJ * BJ) * BK * 2;                               // one step
   static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
-  static constexpr int EXACT = PJ == 3 ? (BI + BJ) * (BK + 1) * 4 : 0;
+  static constexpr int EXACT = PI > 1 ? (BI + BJ) * (BK + 1) * 4 : 0;
   static constexpr int SUMS = OP == BACK_WEIGHT ? NT * 8 * 4 : 0;
   static constexpr int m1 = 2 * BUF > EPI ? 2 * BUF : EPI, m2 = EXACT > SUMS ? EXACT : SUMS, LDS = m1 > m2 ? m1 : m2;
 };
@@ -615,7 +617,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     sixteen(Const<KK - 1>(), No(), No(), buf);
   }
 
-  if (PJ == 3) {
+  if (PI > 1) {                                        // operands in parts
     int bad = 0;
 #pragma unroll
     for (int x = 0; x < NI; ++x)

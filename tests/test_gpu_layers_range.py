@@ -101,3 +101,38 @@ def test_gradients_where_an_activation_is_saturated(m, k, n, act, beta, lo, hi, 
     yb = (big * (0.5 + torch.rand(m, n, generator=gen(4), device="cuda"))).to(dtype)
     xb, wb, bb = ops.linear_backward(yb, x, w, dact, act)
     check_gradients(xb, wb, bb, yb.double() * d, x, w, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("m,k,n", [(200, 70, 130), (16384, 512, 512), (30, 9, 5)])
+def test_infinities_in_gradients_have_the_sign_of_their_product(m, k, n, dtype):
+    """One infinity in x, in the weight or in ybar: every entry it meets is that infinity with the sign of the other factor - which no sum of
+    parts may turn into NaN -, the others are as without it."""
+    g = gen(k)
+    x, w = torch.randn(m, k, generator=g, device="cuda").to(dtype), torch.randn(n, k, generator=g, device="cuda").to(dtype)
+    yb = torch.randn(m, n, generator=g, device="cuda").to(dtype)
+    dact = 0.25 + torch.rand(m, n, generator=g, device="cuda")
+    dact = (dact * 4).round() / 4                          # quarters: some products are exact in one part, some are not
+    yb = torch.where(yb == 0, torch.ones_like(yb), yb)
+    clean = ops.linear_backward(yb, x, w, dact, "silu")
+    zb = yb.double() * dact.double()
+    for what, at in (("x", (m // 2, k - 1)), ("w", (n // 3, k // 2)), ("yb", (m - 1, n // 2))):
+        t = {"x": x, "w": w, "yb": yb}
+        t[what] = t[what].clone()
+        t[what][at] = -math.inf
+        xb, wb, bb = ops.linear_backward(t["yb"], t["x"], t["w"], dact, "silu")
+        inf = lambda s: -math.inf * s.double().sign()
+        if what == "x":
+            want = ((xb, clean[0], None, None), (wb, clean[1], (slice(None), at[1]), inf(zb[at[0]])), (bb, clean[2], None, None))
+        elif what == "w":
+            want = ((xb, clean[0], (slice(None), at[1]), inf(zb[:, at[0]])), (wb, clean[1], None, None), (bb, clean[2], None, None))
+        else:
+            want = ((xb, clean[0], at[0], inf(w[at[1]])), (wb, clean[1], at[1], inf(x[at[0]])), (bb, clean[2], at[1], torch.tensor(-math.inf, device="cuda")))
+        for got, base, where, expect in want:
+            got, base = got.double().clone(), base.double().clone()
+            if where is not None:
+                meets = expect != 0                        # (an infinity times zero is NaN)
+                assert torch.equal(torch.where(expect.isnan(), 0.0, got[where]), torch.where(expect.isnan(), 0.0, expect.double())), what
+                got[where], base[where] = 0.0, 0.0
+            # the tile that met an infinity is summed in float32 instead of in parts: both are within the type's step of the exact sum
+            assert float((got - base).abs().max()) <= 2 * torch.finfo(dtype).eps * float(base.abs().max()) + (m + n) * 8 * U32 * 8, what
