@@ -12,12 +12,17 @@
 //     transpose 4 x 16 blocks on the way to the registers.
 // Both are swizzled by 16- or 64-byte groups so that neither the writes nor the reads of a wave meet in a bank.
 // act' is applied on the way to LDS: zbar is never stored.
-//   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' has more bits than the type.  For NONE and RELU it is exact.  For
-//     the smooth activations 64 x 64 tiles take it as two parts of the type, the rounded value and the rounded rest (16 bits of
-//     bfloat16, 22 of float16), at two products per pair: they are bound by latency, and it costs little (512 x 256 x 256 bf16: dx 6.5
-//     us against 5.7).  The larger tiles, bound by their products, round it once (16 384 x 1 024 x 1 024: 49 us against 98), as every operand
-//     of a 16-bit product is, which makes the gradients' rms error 1.4 times that of rounding them alone.  act' itself is kept in
-//     float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20) keeps all its bits.
+//   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' has more bits than the type, and more range than float16.  For
+//     NONE and RELU it is exact.  For the smooth activations:
+//     bfloat16: 64 x 64 tiles take it as two parts of the type, the rounded value and the rounded rest (16 bits), at two
+//     products per pair: they are bound by latency, and it costs little (512 x 256 x 256 bf16: dx 6.5 us against 5.7).  The larger
+//     tiles, bound by their products, round it once (16 384 x 1 024 x 1 024: 49 us against 98), as every operand of a 16-bit product is,
+//     which makes the gradients' rms error 1.4 times that of rounding them alone.
+//     float16: zbar as two bfloat16 parts (16 bits, float32's range), x and W as two (exact: 11 bits), three products - the rests' product
+//     is below 2^-17 of the pair.  As float16 numbers, products of 2^-12 and 2^-13 would be zero and those past 65 504 infinite,
+//     though their sums fit the type (16 384 x 1 024 x 1 024: dx 108 us, dW 116 against 50 and 66 in float16).
+//     act' itself is kept in float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20)
+//     keeps all its bits.
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
@@ -55,8 +60,10 @@ template <> struct Ty<float> { static constexpr int PLANES = 3; typedef __bf16 L
 template <> struct Ty<_Float16> { static constexpr int PLANES = 1; typedef _Float16 L; typedef f16x8 L8; };
 template <> struct Ty<__bf16> { static constexpr int PLANES = 1; typedef __bf16 L; typedef bf16x8 L8; };
 
-// planes of an operand: the parts it is split into
-template <typename T, int DM> constexpr int planes() { return DM == PARTS ? 2 : Ty<T>::PLANES; }
+// how a product of tensors of type T with A's act' taken as DM is formed: planes (the parts an operand is split into) of A and B, their type
+template <typename T, int DM> struct How : Ty<T> { static constexpr int PI = Ty<T>::PLANES, PJ = PI; };
+template <> struct How<_Float16, PARTS> : Ty<__bf16> { static constexpr int PI = 2, PJ = 2; };
+template <> struct How<__bf16, PARTS> : Ty<__bf16> { static constexpr int PI = 2, PJ = 1; };
 
 template <bool C, typename A, typename B> struct Pick { typedef A type; };
 template <typename A, typename B> struct Pick<false, A, B> { typedef B type; };
@@ -280,10 +287,9 @@ template <typename T> struct Factor<T, MASK> { typedef T type; };
 
 // One operand's step in registers: BA tile rows x BK values in chunks, NC per thread of NT.  SINGLE: a tensor may hold fewer than
 // 16 elements.
-template <typename T, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool SINGLE> struct Stage {
+template <typename T, typename L, int PL, int SRC, int DM, bool PERM, int BA, int BK, int NT, bool SINGLE> struct Stage {
   typedef typename Factor<T, DM>::type Q;
-  typedef typename Ty<T>::L L;
-  static constexpr int PL = planes<T, DM>(), CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
+  static constexpr int CH = BK / 8, CW = BA / 8, NC = BA * BK / 8 / NT;
   typedef Tile<SRC, BA, BK> Tl;
   Chunk<T> v[NC];
   Chunk<Q> q[DM != PLAIN ? NC : 1];
@@ -506,7 +512,7 @@ template <int N> struct Const { constexpr operator int() const { return N; } };
 
 // ---- the tile kernel ---------------------------------------------------------------------------------------------------------
 template <typename T, int OP, int DM, int WI, int WJ, int NI, int NJ, int BK> struct Shape {
-  static constexpr int PI = planes<T, DM>(), PJ = planes<T, PLAIN>(), BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
+  static constexpr int PI = How<T, DM>::PI, PJ = How<T, DM>::PJ, BI = 32 * NI * WI, BJ = 32 * NJ * WJ, NT = 64 * WI * WJ;
   static constexpr int BUF = (PI * BI + PJ * BJ) * BK * 2;                               // one step
   static constexpr int EPITCH = 32 * NJ + 4, EPI = WI * WJ * 32 * EPITCH * 4;       // the tile on its way out
   static constexpr int EXACT = PI > 1 ? (BI + BJ) * (BK + 1) * 4 : 0;
@@ -519,9 +525,10 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
   typedef Shape<T, OP, DM, WI, WJ, NI, NJ, BK> Sh;
   constexpr int SI = OP == BACK_WEIGHT ? COLS : ROWS, SJ = OP == FORWARD ? ROWS : COLS;
   constexpr int PI = Sh::PI, PJ = Sh::PJ, BI = Sh::BI, BJ = Sh::BJ, NT = Sh::NT, EPITCH = Sh::EPITCH, KK = BK / 16;
-  typedef typename Ty<T>::L8 L8;
-  typedef Stage<T, SI, DM, false, BI, BK, NT, SINGLE> StI;
-  typedef Stage<T, SJ, PLAIN, true, BJ, BK, NT, SINGLE> StJ;
+  typedef typename How<T, DM>::L L;
+  typedef typename How<T, DM>::L8 L8;
+  typedef Stage<T, L, PI, SI, DM, false, BI, BK, NT, SINGLE> StI;
+  typedef Stage<T, L, PJ, SJ, PLAIN, true, BJ, BK, NT, SINGLE> StJ;
   extern __shared__ __align__(16) char lds[];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -554,7 +561,7 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
 
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / WJ, wj = wave % WJ;
   f32x16 acc[NI][NJ] = {};
-  constexpr int READS = NI * PI + NJ * PJ, MF = NI * NJ * (PJ == 3 ? 6 : PI);      // per 16 values of the reduction
+  constexpr int READS = NI * PI + NJ * PJ, MF = NI * NJ * (PJ == 3 ? 6 : PI + PJ - 1);      // per 16 values of the reduction
   constexpr int PUT0 = KK > 2 ? KK - 3 : 0, PUTS = KK - 1 - PUT0;              // the sixteens beside which the next step goes to LDS
   static_assert(KK >= 2, "");
   struct Operands { L8 i[NI][PI], j[NJ][PJ]; };
@@ -569,9 +576,10 @@ __global__ __launch_bounds__(64 * WI * WJ, OCC) void tile_kernel(const Args a) {
     else o.j[(b - NI) % NJ][p % PJ] = fragment<L8, SJ, BJ, BK, true>(bj + p * StJ::Tl::BYTES, wj * NJ + b - NI, kk, lane);
   };
   auto product = [&](const Operands& o, int q) {       // the small products first
-    constexpr int QI[6] = {2, 0, 1, 0, 1, 0}, QJ[6] = {0, 2, 1, 1, 0, 0};
+    constexpr int QI[6] = {2, 0, 1, 0, 1, 0}, QJ[6] = {0, 2, 1, 1, 0, 0};      // three parts each: a + b <= 2
+    constexpr int HI[3] = {1, 0, 0}, HJ[3] = {0, 1, 0};                        // two and two: a + b <= 1; two and one
     const int t = q / (NI * NJ), x = q % (NI * NJ) / NJ, y = q % NJ;
-    acc[x][y] = mfma(o.j[y][PJ == 3 ? QJ[t] : 0], o.i[x][PJ == 3 ? QI[t] : PI - 1 - t], acc[x][y]);
+    acc[x][y] = mfma(o.j[y][(PJ == 3 ? QJ[t] : HJ[t]) % PJ], o.i[x][(PJ == 3 ? QI[t] : HI[t]) % PI], acc[x][y]);
   };
   // The kk-th 16 values of a step, and between their MFMAs - in this order, a few instructions after each - the reads of the next
   // sixteen's operands (READ; the last one reads the next step's first, from the other buffer) and pieces of the next step's way to LDS.
@@ -843,19 +851,22 @@ __global__ __launch_bounds__(256) void reduce_kernel(const Args a) {
 // MIDDLE and LARGE, (8 192 x 2 048 x 2 048 f32) 130 and 212 on SMALL and LARGE; small outputs want many small tiles.
 enum Variant { FEW = 0, TINY, SMALL, MIDDLE, LARGE };
 struct Size { int i, j; };
-static Size size_of(int dtype, int v) {
+static Size size_of(int dtype, bool parts, int v) {
   if (v <= SMALL) return {64, 64};
+  if (parts && dtype == F16) return {128, 256};
   if (v == MIDDLE) return {128, 128};                   // 16-bit types
   return dtype == F32 ? Size{256, 128} : Size{256, 256};
 }
 
 // What a launch takes, in microseconds, with w tiles per CU that each reduce L values: start + L max(alone, w each) + (w - 1) tile; and
 // S > 1 splits' parts: JOIN + I J (S PART + LAST).  Fitted (rms 12 %) to 2 034 timings of 20 shapes from 64 x 1 024 x 1 024 to
-// 400 000 x 256 x 256, every variant at 1 to 256 splits; the choice by it is on average 2 % above the best of each.
+// 400 000 x 256 x 256, every variant at 1 to 256 splits; the choice by it is on average 2 % above the best of each.  (Gradients in parts:
+// 748 timings of 18 shapes, rms 10 %, 1 %.)
 struct Cost { float start, alone, each, tile; };
 static Cost cost_of(int dtype, bool act_bar, bool parts, int v) {
   if (v == TINY) return {4.0f, 0.036f, 0.006f, 0.30f};
   if (dtype == F32) return v <= SMALL ? Cost{4.0f, 0.0234f, 0.0156f, 0.31f} : Cost{7.9f, 0.0388f, 0.0644f, 7.6f};
+  if (parts && dtype == F16) return v <= SMALL ? Cost{4.34f, 0.0155f, 0.0110f, 0.82f} : Cost{7.92f, 0.0137f, 0.0426f, 5.18f};
   if (v <= SMALL && parts) return {3.95f, 0.0141f, 0.0088f, 0.28f};
   if (v <= SMALL) return act_bar ? Cost{3.6f, 0.0109f, 0.0065f, 0.18f} : Cost{3.4f, 0.0092f, 0.0042f, 0.46f};
   if (v == MIDDLE) return act_bar ? Cost{5.6f, 0.0121f, 0.0164f, 0.60f} : Cost{5.75f, 0.0011f, 0.0121f, 0.89f};
@@ -874,16 +885,16 @@ static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
   Plan p = {};
   p.S = 1;
   if (op == FORWARD && I <= 8) return p;                // FEW
-  const bool act_bar = op != FORWARD && act != NONE;
+  const bool act_bar = op != FORWARD && act != NONE, parts = act_bar && act != RELU && dtype != F32;
   const ll steps = R > 0 ? (R + CHUNK - 1) / CHUNK : 1; // R = 0: the gradient of no rows, one pass over nothing
   // Loaded one by one: operands of less than two chunks, reductions that end inside the first chunk (305 747 x 2 x 20 bf16 16 us against
   // 24) and columns that do (the weight gradient of 510 170 x 50 x 3 f16 34 us against 41: chunks would read on into the rows behind).
   const bool tiny = R < 8 || I * R < 16 || J * R < 16 || (op != FORWARD && J < 8) || (op == BACK_WEIGHT && I < 8);
   float best = 0.0f;
   for (int v = tiny ? TINY : SMALL; v <= (tiny ? TINY : LARGE); ++v) {
-    if (v == MIDDLE && dtype == F32) continue;
-    const Size z = size_of(dtype, v);
-    const Cost c = cost_of(dtype, act_bar, act_bar && act != RELU, v);
+    if (v == MIDDLE && (dtype == F32 || (parts && dtype == F16))) continue;
+    const Size z = size_of(dtype, parts, v);
+    const Cost c = cost_of(dtype, act_bar, parts, v);
     const ll TI = (I + z.i - 1) / z.i, TJ = (J + z.j - 1) / z.j;
     for (int s = 1; s <= MOST && s <= steps; s = s < 4 ? s + 1 : s + (s & (s - 1) ? s / 3 : s / 2)) {      // 1 2 3 4 6 8 12 16 ..
       const ll chunk = (steps + s - 1) / s, S = (steps + chunk - 1) / chunk, n = TI * TJ * S;
@@ -933,6 +944,9 @@ template <typename T, int OP, int DM> static int start_tile(const Args& a, int v
   if constexpr (sizeof(T) == 4) {
     if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 32, 2>(a, grid, st);
     return start<T, OP, DM, 4, 2, 2, 2, 32, 2>(a, grid, st);
+  } else if constexpr (How<T, DS>::PJ == 2) {
+    if (variant == SMALL) return start<T, OP, DS, 2, 2, 1, 1, 64, 2>(a, grid, st);
+    return start<T, OP, DS, 2, 4, 2, 2, 32, 2>(a, grid, st);      // (a step of 64 is more than LDS holds)
   } else {
     if (variant == SMALL) return start<T, OP, DS, 2, 2, 1, 1, 64, 2>(a, grid, st);
     if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, DM == PLAIN ? 64 : 32, 2>(a, grid, st);      // (act' takes registers)
