@@ -14,15 +14,15 @@
 // act' is applied on the way to LDS: zbar is never stored.
 //   * 16-bit types: v_mfma_f32_32x32x16_{f16,bf16}.  zbar = ybar act' has more bits than the type, and more range than float16.  For
 //     NONE and RELU it is exact.  For the smooth activations:
-//     bfloat16: 64 x 64 tiles take it as two parts of the type, the rounded value and the rounded rest (16 bits), at two
-//     products per pair: they are bound by latency, and it costs little (512 x 256 x 256 bf16: dx 6.5 us against 5.7).  The larger
-//     tiles, bound by their products, round it once (16 384 x 1 024 x 1 024: 49 us against 98), as every operand of a 16-bit product is,
-//     which makes the gradients' rms error 1.4 times that of rounding them alone.
+//     bfloat16: two parts of the type, the rounded value and the rounded rest (16 bits), and two products, whatever the tile: the same
+//     rows have the same precision in every batch.  Rounded once, the gradients' rms error was 1.4 times that of rounding the outputs
+//     alone, at 49 us for dx of 16 384 x 1 024 x 1 024 against 77 (dW 68 against 84) and 20 against 25 of 16 384 x 512 x 512.
 //     float16: zbar as two bfloat16 parts (16 bits, float32's range), x and W as two (exact: 11 bits), three products - the rests' product
 //     is below 2^-17 of the pair.  As float16 numbers, products of 2^-12 and 2^-13 would be zero and those past 65 504 infinite,
 //     though their sums fit the type (16 384 x 1 024 x 1 024: dx 108 us, dW 116 against 50 and 66 in float16).
 //     act' itself is kept in float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20)
-//     keeps all its bits.
+//     keeps all its bits.  In parts, tiles are 128 x 256 (A, which is formed from two tensors, for as many columns as possible: 256 x 128 take 97 us
+//     where these take 77, 256 x 256 do not fit the registers).
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
 //     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
@@ -853,7 +853,7 @@ enum Variant { FEW = 0, TINY, SMALL, MIDDLE, LARGE };
 struct Size { int i, j; };
 static Size size_of(int dtype, bool parts, int v) {
   if (v <= SMALL) return {64, 64};
-  if (parts && dtype == F16) return {128, 256};
+  if (parts) return {128, 256};
   if (v == MIDDLE) return {128, 128};                   // 16-bit types
   return dtype == F32 ? Size{256, 128} : Size{256, 256};
 }
@@ -867,7 +867,7 @@ static Cost cost_of(int dtype, bool act_bar, bool parts, int v) {
   if (v == TINY) return {4.0f, 0.036f, 0.006f, 0.30f};
   if (dtype == F32) return v <= SMALL ? Cost{4.0f, 0.0234f, 0.0156f, 0.31f} : Cost{7.9f, 0.0388f, 0.0644f, 7.6f};
   if (parts && dtype == F16) return v <= SMALL ? Cost{4.34f, 0.0155f, 0.0110f, 0.82f} : Cost{7.92f, 0.0137f, 0.0426f, 5.18f};
-  if (v <= SMALL && parts) return {3.95f, 0.0141f, 0.0088f, 0.28f};
+  if (parts) return v <= SMALL ? Cost{4.48f, 0.0134f, 0.0085f, 0.40f} : Cost{7.83f, 0.0228f, 0.0278f, 6.02f};
   if (v <= SMALL) return act_bar ? Cost{3.6f, 0.0109f, 0.0065f, 0.18f} : Cost{3.4f, 0.0092f, 0.0042f, 0.46f};
   if (v == MIDDLE) return act_bar ? Cost{5.6f, 0.0121f, 0.0164f, 0.60f} : Cost{5.75f, 0.0011f, 0.0121f, 0.89f};
   return act_bar ? Cost{8.3f, 0.0093f, 0.0343f, 7.2f} : Cost{8.2f, 0.0040f, 0.0295f, 7.1f};
@@ -892,7 +892,7 @@ static Plan plan(int op, int dtype, int act, ll I, ll J, ll R) {
   const bool tiny = R < 8 || I * R < 16 || J * R < 16 || (op != FORWARD && J < 8) || (op == BACK_WEIGHT && I < 8);
   float best = 0.0f;
   for (int v = tiny ? TINY : SMALL; v <= (tiny ? TINY : LARGE); ++v) {
-    if (v == MIDDLE && (dtype == F32 || (parts && dtype == F16))) continue;
+    if (v == MIDDLE && (dtype == F32 || parts)) continue;
     const Size z = size_of(dtype, parts, v);
     const Cost c = cost_of(dtype, act_bar, parts, v);
     const ll TI = (I + z.i - 1) / z.i, TJ = (J + z.j - 1) / z.j;
@@ -944,11 +944,11 @@ template <typename T, int OP, int DM> static int start_tile(const Args& a, int v
   if constexpr (sizeof(T) == 4) {
     if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 32, 2>(a, grid, st);
     return start<T, OP, DM, 4, 2, 2, 2, 32, 2>(a, grid, st);
-  } else if constexpr (How<T, DS>::PJ == 2) {
+  } else if constexpr (DS == PARTS) {
     if (variant == SMALL) return start<T, OP, DS, 2, 2, 1, 1, 64, 2>(a, grid, st);
-    return start<T, OP, DS, 2, 4, 2, 2, 32, 2>(a, grid, st);      // (a step of 64 is more than LDS holds)
+    return start<T, OP, DS, 2, 4, 2, 2, How<T, DS>::PJ == 1 ? 64 : 32, 2>(a, grid, st);      // (float16: 64 is more than LDS holds)
   } else {
-    if (variant == SMALL) return start<T, OP, DS, 2, 2, 1, 1, 64, 2>(a, grid, st);
+    if (variant == SMALL) return start<T, OP, DM, 2, 2, 1, 1, 64, 2>(a, grid, st);
     if (variant == LARGE) return start<T, OP, DM, 2, 4, 4, 2, DM == PLAIN ? 64 : 32, 2>(a, grid, st);      // (act' takes registers)
     return start<T, OP, DM, 2, 2, 2, 2, 64, 2>(a, grid, st);
   }
