@@ -83,11 +83,15 @@ class EmbeddingHip(torch.autograd.Function):
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
            activation: str = "none", beta: float = 100.0) -> torch.Tensor:
     """``ops.linear`` with gradients for x, weight, bias and residual."""
+    if not torch.is_grad_enabled():      # (inside the Function it always is off, and needs_input_grad is requires_grad alone)
+        return ops.linear(x, weight, bias, residual, activation, float(beta))
     return LinearHip.apply(x, weight, bias, residual, activation, float(beta))
 
 
 def embedding(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``ops.embedding`` with the table's gradient."""
+    if not torch.is_grad_enabled():
+        return ops.embedding(table, index, float(scale))
     return EmbeddingHip.apply(table, index, float(scale))
 
 
