@@ -47,7 +47,7 @@ class LinearHip(torch.autograd.Function):
             return ops.linear(x, weight, bias, residual, activation, beta)
         _same_side_of_capture(x, weight, bias, residual)
         y, dact = ops.linear_train_forward(x, weight, bias, residual, activation, beta)
-        ctx.save_for_backward(x, weight, dact)      # relu without residual: dact is y, an output (saved as such, no copy)
+        ctx.save_for_backward(x, weight, dact)      # relu without residual: dact may be y, an output (saved as such, no copy)
         ctx.activation = activation
         return y
 

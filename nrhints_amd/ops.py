@@ -389,16 +389,17 @@ def _linear_forward(x, weight, bias, residual, activation, beta, want_dact):
         r2, ldr = _matrix(residual, m, n, x, "residual")
     y = x.new_empty(shape)
     dact = None
-    if want_dact and code != 0 and not (code == 1 and residual is None):
+    # ReLU without a residual: y is positive exactly where the argument is (bfloat16: down to 2^-134 of it) and serves as the mask - not in
+    # float16, where arguments up to 2^-25 round to zero
+    masks_itself = code == 1 and residual is None and x.dtype != torch.float16
+    if want_dact and code != 0 and not masks_itself:
         dact = x.new_empty(shape, dtype=x.dtype if code == 1 else torch.float32)
     ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 0, dtype, code, m, n, k)
     with _Here(x.device) as stream:
         rc = _lib.load().nrh_linear_forward(dtype, x2.data_ptr(), ldx, w2.data_ptr(), ldw, _vp(b1), _vp(r2), ldr, code, beta, m, n, k,
                                             y.data_ptr(), n, _vp(dact), _vp(ws), nbytes, stream)
     _lib.check(rc, "nrh_linear_forward")
-    if want_dact and code == 1 and residual is None:
-        dact = y           # ReLU: the output is positive exactly where the argument is
-    return y, dact
+    return y, (y if want_dact and masks_itself else dact)
 
 
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
@@ -414,7 +415,8 @@ def linear_train_forward(x: torch.Tensor, weight: torch.Tensor, bias: Optional[t
                          residual: Optional[torch.Tensor] = None, activation: str = "none",
                          beta: float = 100.0) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``linear`` that also keeps what its gradient needs: -> (y, dact), dact = act'(x weight^T + bias) in float32, None for
-    "none", a mask of x's type for "relu": y itself where there is no residual (do not change y in place before the backward then)."""
+    "none", a mask of x's type for "relu": y itself where there is no residual and the type is not float16 (do not change y in place before the
+    backward then)."""
     return _linear_forward(x, weight, bias, residual, activation, beta, True)
 
 

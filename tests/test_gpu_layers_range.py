@@ -188,3 +188,23 @@ def test_gradients_have_one_precision_in_every_batch(act, dtype):
             own = (got.double() - want).norm() / want.norm()
             alone = (want.to(dtype).double() - want).norm() / want.norm()
             assert dtype == torch.float32 or float(own) <= 1.05 * float(alone), (name, rows, float(own), float(alone))
+
+
+@pytest.mark.parametrize("dtype", DT, ids=IDS)
+@pytest.mark.parametrize("m", [3, 200])
+def test_relu_passes_gradients_of_arguments_that_round_to_zero(m, dtype):
+    """z = 2^-26 is positive, y = relu(z) is 0 in float16: the gradient passes all the same, with a residual and without."""
+    x, w = torch.full((m, 16), 2.0 ** -15, dtype=dtype, device="cuda"), torch.full((24, 16), 2.0 ** -15, dtype=dtype, device="cuda")
+    w[12:] = -w[12:]
+    yb = torch.randn(m, 24, generator=gen(2), device="cuda").to(dtype)
+    zero = torch.zeros(m, 24, dtype=dtype, device="cuda")
+    plain, beside = (ops.linear_train_forward(x, w, None, r, "relu") for r in (None, zero))
+    if dtype == torch.float16:
+        assert not plain[0].any()
+    on = torch.where(torch.arange(24, device="cuda") < 12, yb, torch.zeros_like(yb))
+    for _, mask in (plain, beside):
+        xb, wb, bb = ops.linear_backward(yb, x, w, mask, "relu")
+        check_gradients(xb, wb, bb, on.double(), x, w, dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+    grads = torch.autograd.grad(layers.linear(*leaves, activation="relu"), leaves, yb)
+    check_gradients(*grads, None, on.double(), x, w, dtype)
