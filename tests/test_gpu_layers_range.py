@@ -2,8 +2,8 @@
 
 u32 = 2^-24.  Arguments are one product with 1, so they are exact; act' is then off by at most 24 u32 of its value: 2 for the exponential,
 6 for the complementary error function, 1 for every other step of at most ten, and (softplus) 4 for log or division by beta - never by an
-absolute amount.  ybar act' as an operand of a 16-bit product: two bfloat16 parts leave out at most 2^-17 of it and the low parts' product
-2^-18 (2^-16 together).  Float32 sums of R terms add (R + 8) u32 of the sum of magnitudes, twice
+absolute amount.  ybar act' as an operand of a 16-bit product: two bfloat16 parts leave out at most 2^-16 of it (half a step of a rest of
+2^-8) and, where x and the weight are in parts too (float16), the rests' product 2^-16.  Float32 sums of R terms add (R + 8) u32 of the sum of magnitudes, twice
 that in two parts; an output is rounded once (float16: half a subnormal step, 2^-25, at least)."""
 import math
 
@@ -17,7 +17,7 @@ from nrhints_amd import layers, ops  # noqa: E402
 U32 = 2.0 ** -24
 DT = [torch.float32, torch.float16, torch.bfloat16]
 IDS = ["f32", "f16", "bf16"]
-LEFT_OUT = {torch.float32: 0.0, torch.float16: 2.0 ** -16, torch.bfloat16: 2.0 ** -16}
+LEFT_OUT = {torch.float32: 0.0, torch.float16: 2.0 ** -15, torch.bfloat16: 2.0 ** -16}
 LOWEST = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}
 
 
@@ -181,7 +181,7 @@ def test_gradients_have_one_precision_in_every_batch(act, dtype):
     for rows in (m, 200):
         xb, wb, _ = ops.linear_backward(yb[:rows], x[:rows], w, dact[:rows], act)
         zb, X, W = yb[:rows].double() * dact[:rows].double(), x[:rows].double(), w.double()
-        rel, ut = (0.0 if dtype == torch.float32 else 2.0 ** -16), torch.finfo(dtype).eps / 2
+        rel, ut = LEFT_OUT[dtype], torch.finfo(dtype).eps / 2
         for name, got, want, size, r in (("x", xb, zb @ W, zb.abs() @ W.abs(), n), ("w", wb, zb.t() @ X, zb.abs().t() @ X.abs(), rows)):
             within(name, got, want, (rel + (2 * r + 8) * U32) * size + 1.01 * ut * want.abs() + LOWEST[dtype])
             # ... and the rms error is that of rounding exact values to the type, up to a twentieth
@@ -208,3 +208,23 @@ def test_relu_passes_gradients_of_arguments_that_round_to_zero(m, dtype):
     leaves = [t.clone().requires_grad_(True) for t in (x, w)]
     grads = torch.autograd.grad(layers.linear(*leaves, activation="relu"), leaves, yb)
     check_gradients(*grads, None, on.double(), x, w, dtype)
+
+
+def test_many_rows_past_32_bits():
+    """2^31 elements and more behind one operand with many rows: the last of 600 000 rows of 4 100 elements, bit for bit what the same rows
+    give by themselves in a launch of as many tiles, and within the bound of a bfloat16 product."""
+    m, ld, k, n = 600000, 4100, 96, 40
+    big = torch.zeros(m, ld, dtype=torch.bfloat16, device="cuda")
+    assert big.numel() > 2 ** 31
+    g = gen(1)
+    x = big[:, 2000:2000 + k]
+    x.copy_(torch.randn(m, k, generator=g, device="cuda"))
+    w = torch.randn(n, k, generator=g, device="cuda").bfloat16()
+    y = ops.linear(x, w)
+    assert torch.equal(y, ops.linear(x.contiguous(), w))
+    want, size = x[-300:].double() @ w.double().t(), x[-300:].double().abs() @ w.double().abs().t()
+    within("y", y[-300:], want, (k + 8) * U32 * size + 1.01 * 2.0 ** -8 * want.abs())
+    yb = torch.randn(m, n, generator=g, device="cuda").bfloat16()
+    _, wb, _ = ops.linear_backward(yb, x, w, None)
+    want, size = yb.double().t() @ x.double(), yb.double().abs().t() @ x.double().abs()
+    within("w", wb, want, (m + 8) * U32 * size + 1.01 * 2.0 ** -8 * want.abs())
