@@ -18,15 +18,16 @@
 //     rows have the same precision in every batch.  Rounded once, the gradients' rms error was 1.4 times that of rounding the outputs
 //     alone, at 49 us for dx of 16 384 x 1 024 x 1 024 against 77 (dW 68 against 84) and 20 against 25 of 16 384 x 512 x 512.
 //     float16: zbar as two bfloat16 parts (16 bits, float32's range), x and W as two (exact: 11 bits), three products - the rests' product
-//     is below 2^-17 of the pair.  As float16 numbers, products of 2^-12 and 2^-13 would be zero and those past 65 504 infinite,
+//     is at most 2^-16 of the pair.  As float16 numbers, products of 2^-12 and 2^-13 would be zero and those past 65 504 infinite,
 //     though their sums fit the type (16 384 x 1 024 x 1 024: dx 108 us, dW 116 against 50 and 66 in float16).
 //     act' itself is kept in float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20)
 //     keeps all its bits.  In parts, tiles are 128 x 256 (A, which is formed from two tensors, for as many columns as possible: 256 x 128 take 97 us
 //     where these take 77, 256 x 256 do not fit the registers).
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
-//     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is below 2^-25 of |x w|, under float32's own rounding; six
-//     passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has float32's exponent range, so nothing
-//     is scaled.
+//     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is at most 2^-23 of |x w|, two of float32's own half steps
+//     (x1 w2 and x2 w1, 2^-24 each); six passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has
+//     float32's exponents, so nothing is scaled; but its numbers end at 2^-133, float32's at 2^-149: below 2^-109 the parts leave out up
+//     to 2^-134 of x itself.
 // Operands in parts: infinities, NaN and values that round up to infinity make the parts NaN, and an infinity on the other side
 // meets parts that are zero or of the other sign.  A tile whose sums are not all finite is computed again with
 // v_mfma_f32_32x32x2_f32, so its results are those of float32 arithmetic.

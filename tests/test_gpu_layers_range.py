@@ -228,3 +228,16 @@ def test_many_rows_past_32_bits():
     _, wb, _ = ops.linear_backward(yb, x, w, None)
     want, size = yb.double().t() @ x.double(), yb.double().abs().t() @ x.double().abs()
     within("w", wb, want, (m + 8) * U32 * size + 1.01 * 2.0 ** -8 * want.abs())
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -112, 2.0 ** -120, 2.0 ** -126])
+def test_float32_products_of_very_small_numbers(scale):
+    """The three bfloat16 parts of a float32 number end at 2^-133, bfloat16's smallest: what they leave out of x is at most 2^-134, below
+    2^-25 of it down to 2^-109, and each product misses at most that times |w|."""
+    g = gen(6)
+    m, k, n = 300, 200, 140
+    x, w = torch.randn(m, k, generator=g, device="cuda") * scale, torch.randn(n, k, generator=g, device="cuda")
+    X, W = x.double(), w.double()
+    size = X.abs() @ W.abs().t()
+    bound = (k + 8) * U32 * size + 2.0 ** -134 * W.abs().sum(1) + k * 2.0 ** -149
+    within("y", ops.linear(x, w), X @ W.t(), bound)
