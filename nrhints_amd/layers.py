@@ -4,8 +4,8 @@ csrc/nrh_embedding.hip).
 The networks of the renderer run on kernels whose shape is compiled in; these are the building blocks for networks that have another
 one (the background network at other widths and depths, outside.OutsideNeRF) and for tables looked up per ray (RayGenerator's
 per-view deltas).  GPU tensors only, float32 / float16 / bfloat16, one derivative (a second one raises).  Gradients are summed in a
-fixed order: the same bits on every run.  Forward and backward may be captured into a graph; a capture is refused while an eager graph
-of the same parameters is alive.
+fixed order: the same bits on every run.  Forward and backward may be captured into a graph; a capture is refused while a graph of
+the same parameters that was recorded on another stream is alive.
 """
 from __future__ import annotations
 
@@ -20,22 +20,32 @@ from torch.autograd.graph import get_gradient_edge
 from . import ops
 
 
-_EAGER = "nrhints_amd.layers: recorded outside a capture"
+_STREAM = "nrhints_amd.layers: stream"
 
 
-def _same_side_of_capture(*tensors) -> None:
-    """A parameter's gradient is accumulated on the stream its graph was first recorded on.  If an eager graph of the parameter is still
-    alive, a backward pass captured now would accumulate on the eager stream and end the process: refuse it here, while an exception
-    still can."""
+def _same_side_of_capture(*tensors) -> list:
+    """A parameter's gradient is accumulated on the stream on which its accumulation node was made, by the first graph that holds the
+    parameter, and the node lives as long as any graph does.  A backward pass captured on another stream would accumulate outside the
+    capture and end the process: refuse it here, while an exception still can.  -> the nodes, to be held until the graph holds them."""
+    held = []
     for t in tensors:
-        if t is not None and t.is_cuda and t.requires_grad and t.is_leaf:
-            capturing = torch.cuda.is_current_stream_capturing()
-            meta = get_gradient_edge(t).node.metadata
-            if not capturing:
-                meta[_EAGER] = True
-            elif _EAGER in meta:
-                raise RuntimeError("a graph recorded outside this capture still holds one of these parameters: delete its outputs "
-                                   "(or detach them) before capturing")
+        if not (isinstance(t, torch.Tensor) and t.is_cuda and t.requires_grad and t.is_leaf):
+            continue
+        capturing, here = torch.cuda.is_current_stream_capturing(), torch._C._cuda_getCurrentRawStream(t.device.index)
+        node = get_gradient_edge(t).node
+        if _STREAM not in node.metadata:
+            # Made here and now, it dies with its last reference.  One that stays belongs to another operation's graph: to this capture's own, as far
+            # as can be told, or outside a capture to a stream that nobody knows.
+            node.metadata[_STREAM] = here if capturing else None
+            del node
+            node = get_gradient_edge(t).node
+            node.metadata.setdefault(_STREAM, here)
+        if capturing and node.metadata[_STREAM] != here:
+            raise RuntimeError("a graph recorded outside this capture still holds one of these parameters, on another stream: delete its outputs "
+                               "(or detach them) before capturing, or record it on the capturing stream (as for a wrapper that keeps its "
+                               "parameters' nodes)")
+        held.append(node)
+    return held
 
 
 class LinearHip(torch.autograd.Function):
@@ -45,7 +55,6 @@ class LinearHip(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation: str, beta: float):
         if not any(ctx.needs_input_grad[:3]):
             return ops.linear(x, weight, bias, residual, activation, beta)
-        _same_side_of_capture(x, weight, bias, residual)
         y, dact = ops.linear_train_forward(x, weight, bias, residual, activation, beta)
         ctx.save_for_backward(x, weight, dact)      # relu without residual: dact may be y, an output (saved as such, no copy)
         ctx.activation = activation
@@ -67,8 +76,6 @@ class EmbeddingHip(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, index, scale: float):
-        if ctx.needs_input_grad[0]:
-            _same_side_of_capture(table)
         ctx.save_for_backward(index)
         ctx.rows, ctx.scale = table.shape[0], float(scale)
         return ops.embedding(table, index, scale)
@@ -85,6 +92,7 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     """``ops.linear`` with gradients for x, weight, bias and residual."""
     if not torch.is_grad_enabled():      # (inside the Function it always is off, and needs_input_grad is requires_grad alone)
         return ops.linear(x, weight, bias, residual, activation, float(beta))
+    held = _same_side_of_capture(x, weight, bias, residual)      # noqa: F841 - until the Function's node holds them
     return LinearHip.apply(x, weight, bias, residual, activation, float(beta))
 
 
@@ -92,6 +100,7 @@ def embedding(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> t
     """``ops.embedding`` with the table's gradient."""
     if not torch.is_grad_enabled():
         return ops.embedding(table, index, float(scale))
+    held = _same_side_of_capture(table)      # noqa: F841 - until the Function's node holds it
     return EmbeddingHip.apply(table, index, float(scale))
 
 

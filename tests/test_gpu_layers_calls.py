@@ -62,3 +62,79 @@ def test_an_inference_is_captured_beside_a_live_eager_graph():
         second.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(want, g1, g2))
+
+
+def test_a_capture_on_the_stream_of_a_live_eager_graph():
+    """Parameters whose eager graph lives on the capturing stream accumulate their gradients on that stream: nothing to refuse (a wrapper that
+    keeps its parameters' accumulation nodes captures this way)."""
+    net, view, seed = net_and_batch()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = net(view)
+        alive.backward(seed, retain_graph=True)
+        want = [p.grad.clone() for p in net.parameters()]
+        net.zero_grad()
+    torch.cuda.synchronize()
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        net(view).backward(seed)
+    grads = [p.grad for p in net.parameters()]
+    for _ in range(3):
+        for t in grads:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, grads))
+    assert alive.grad_fn is not None
+    # ... and on another stream, beside the graph recorded in the first capture's stream: refused
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=other):
+            net(view)
+    torch.cuda.synchronize()
+
+
+def test_two_captures_on_two_streams_with_the_first_ones_graph_alive():
+    """The nodes of a graph recorded by a capture belong to its stream: a capture on another one is refused while they live."""
+    net, view, seed = net_and_batch()
+    with torch.no_grad():
+        net(view)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=streams[0]):
+        held = net(view)
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=streams[1]):
+            net(view)
+    torch.cuda.synchronize()
+    del held
+
+
+def test_a_capture_beside_another_operations_graph_is_refused():
+    """A graph that another operation recorded on a stream of its own holds the parameters first: the layers see its node in their warm-up and
+    refuse the capture that would accumulate there; inside a capture another operation on the same parameters is no matter."""
+    net, view, seed = net_and_batch()
+    penalty = sum((p * p).sum() for p in net.parameters())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        net(view)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="outside this capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            net(view)
+    torch.cuda.synchronize()
+    del penalty
+    want = torch.autograd.grad(net(view), list(net.parameters()), seed)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr, stream=side):
+        twice = [p * 2 for p in net.parameters()]
+        grads = torch.autograd.grad(net(view), list(net.parameters()), seed)
+    for _ in range(3):
+        for t in grads:
+            t.zero_()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, grads)) and all(torch.equal(t, p * 2) for t, p in zip(twice, net.parameters()))
