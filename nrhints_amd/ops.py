@@ -434,7 +434,9 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
     d2, ldd = (None, 0) if dact is None else _matrix(dact, m, n, x, "dact", x.dtype if code == 1 else torch.float32)
     lib = _lib.load()
     x_bar = x.new_empty(x.shape) if want_x else None
-    w_bar = x.new_empty((n, k)) if (want_weight or want_bias) else None
+    # (a bias alone: the column sums of ybar act' beside the weight gradient of one column of x)
+    kw = k if want_weight else 1
+    w_bar = x.new_empty((n, kw)) if (want_weight or want_bias) else None
     b_bar = x.new_empty((n,)) if want_bias else None
     with _Here(x.device) as stream:
         if want_x:
@@ -442,9 +444,9 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
             _lib.check(lib.nrh_linear_backward_data(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, w2.data_ptr(), ldw, m, n, k,
                                                     x_bar.data_ptr(), k, _vp(ws), nbytes, stream), "nrh_linear_backward_data")
         if w_bar is not None:
-            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 2, dtype, code, m, n, k)
-            _lib.check(lib.nrh_linear_backward_weight(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, x2.data_ptr(), ldx, m, n, k,
-                                                      w_bar.data_ptr(), k, _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
+            ws, nbytes = _workspace(x, "nrh_linear_workspace_bytes", 2, dtype, code, m, n, kw)
+            _lib.check(lib.nrh_linear_backward_weight(dtype, g2.data_ptr(), ldg, _vp(d2), ldd, code, x2.data_ptr(), ldx, m, n, kw,
+                                                      w_bar.data_ptr(), kw, _vp(b_bar), _vp(ws), nbytes, stream), "nrh_linear_backward_weight")
     return x_bar, (w_bar if want_weight else None), b_bar
 
 

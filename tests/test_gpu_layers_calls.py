@@ -138,3 +138,35 @@ def test_a_capture_beside_another_operations_graph_is_refused():
         gr.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(want, grads)) and all(torch.equal(t, p * 2) for t, p in zip(twice, net.parameters()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("act", ["none", "relu", "silu"])
+def test_a_bias_gradient_alone_leaves_out_the_weights(act, dtype):
+    """Only the bias is trained: its gradient is right and the [n, k] product is neither formed nor allocated."""
+    m, k, n = 3000, 1500, 700
+    g = gen(1)
+    x, w, b = (torch.randn(*s, generator=g, device="cuda").to(dtype) for s in ((m, k), (n, k), (n,)))
+    yb = torch.randn(m, n, generator=g, device="cuda").to(dtype)
+    y, dact = ops.linear_train_forward(x, w / 40, b, None, act)
+    full = ops.linear_backward(yb, x, w, dact, act)
+    only = ops.linear_backward(yb, x, w, dact, act, want_x=False, want_weight=False)
+    assert only[0] is None and only[1] is None
+    d = 1.0 if dact is None else ((dact > 0).double() if act == "relu" else dact.double())
+    zb = yb.double() * d
+    u32 = 2.0 ** -24
+    bound = (m + 8) * u32 * zb.abs().sum(0) + 1.01 * torch.finfo(dtype).eps / 2 * zb.sum(0).abs() + 2.0 ** -25
+    for got in (only[2], full[2]):
+        assert got.shape == (n,) and bool(((got.double() - zb.sum(0)).abs() <= bound).all())
+    assert all(torch.equal(only[2], ops.linear_backward(yb, x, w, dact, act, want_x=False, want_weight=False)[2]) for _ in range(3))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.linear_backward(yb, x, w, dact, act, want_x=False, want_weight=False)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before < n * k * x.element_size()
+    # through autograd: a layer of which only the bias learns
+    bl = b.clone().requires_grad_(True)
+    (gb,) = torch.autograd.grad(layers.linear(x, w / 40, bl, activation=act), bl, yb)
+    assert torch.equal(gb, only[2])
