@@ -646,7 +646,7 @@ int nrh_sdf32_tables(const float* const* sdf_bias, const int* rows, const float*
  *
  * nrh_linear_forward   y [m,n] = act(x [m,k] w [n,k]^T + bias [n]) + residual [m,n]; bias, residual may be null.  activation: 0 none,
  *   1 ReLU, 2 softplus log(1 + exp(beta z)) / beta, 3 sigmoid, 4 SiLU z sigmoid(z), 5 GELU (erf form).  dact [m,n] (contiguous, may be
- *   null): act'(z), what the backward entries need - float32 beside every type (a saturated unit's act' is far below float16's range and
+ *   null and is for activation 0): act'(z), what the backward entries need - float32 beside every type (a saturated unit's act' is far below float16's range and
  *   its gradient need not be); for ReLU 1 or 0 in the tensors' type.  float32 products are six bfloat16 MFMAs over three-way split operands:
  *   at most 2^-23 of each |x w| is left out, and up to 2^-134 of an |x| (or |w|) below 2^-109, where bfloat16's numbers end before
  *   float32's; tiles with infinities or NaN are computed with float32 MFMAs.

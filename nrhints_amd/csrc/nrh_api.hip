@@ -1880,6 +1880,7 @@ int nrh_linear_forward(int dtype, const void* x, long long ldx, const void* w, l
   if (rc) return rc;
   if (m == 0) return NRH_OK;
   if (!x || !w || !y) return fail(NRH_E_INVALID, "%s: null pointer", who);
+  if (dact && activation == nrhlin::NONE) return fail(NRH_E_INVALID, "%s: there is no derivative to keep without an activation", who);
   if (ldx < k || ldw < k || ldy < n || (residual && ldr < n)) return fail(NRH_E_INVALID, "%s: a row stride is smaller than the row", who);
   if (activation == nrhlin::SOFTPLUS && !(beta > 0.0f && beta < 1e30f)) return fail(NRH_E_INVALID, "%s: softplus needs a positive beta", who);
   if (off_element(x, dtype) || off_element(w, dtype) || off_element(y, dtype) || off_element(bias, dtype) || off_element(residual, dtype) ||

@@ -1,9 +1,10 @@
-"""Which entry of the operators a layer takes, told without a GPU."""
+"""What of the layer operators' calls can be told without a GPU: which entry a layer takes, and what the C entries refuse."""
+import ctypes
 
 import pytest
 import torch
 
-from nrhints_amd import layers, ops
+from nrhints_amd import _lib, layers, ops
 
 
 @pytest.fixture
@@ -42,3 +43,13 @@ def test_without_gradients_a_layer_keeps_nothing_for_them(calls, mode):
     for p in lin.parameters():
         p.requires_grad_(False)
     assert not lin(x).requires_grad and calls[4:] == ["linear"]
+
+
+def test_a_derivative_of_no_activation_is_refused():
+    """act' of "none" is one and is not written: a buffer for it is a mistake of the caller's, in every form of the product."""
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(4096 + 16)
+    p = (ctypes.addressof(buf) + 15) // 16 * 16            # never reached by a launch
+    for m in (4, 100):
+        assert lib.nrh_linear_forward(0, p, 8, p, 8, None, None, 0, 0, 1.0, m, 4, 8, p, 4, p, None, 0, None) == -1
+        assert b"activation" in lib.nrh_last_error_string()
