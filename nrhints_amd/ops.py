@@ -306,6 +306,8 @@ def _matrix(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, what: str
     view where the strides allow it (a column block of a wider buffer), else a copy."""
     if not isinstance(t, torch.Tensor) or t.dtype != (dtype or like.dtype) or t.device != like.device:
         raise ValueError(f"{what}: expected a {dtype or like.dtype} tensor on {like.device}, got {getattr(t, 'dtype', type(t))} on {getattr(t, 'device', None)}")
+    if t.is_neg():                                         # (an imaginary part of a conjugate: the sign is a flag of the view)
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t, cols
     if t.dim() != 2:
@@ -453,7 +455,7 @@ def linear_backward(y_bar: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, 
 def _index(index, like, what):
     if not isinstance(index, torch.Tensor) or index.dtype not in (torch.int32, torch.int64) or index.device != like.device:
         raise ValueError(f"{what}: the index must be an int32 or int64 tensor on {like.device}")
-    return index.contiguous(), 64 if index.dtype == torch.int64 else 32
+    return index.resolve_neg().contiguous(), 64 if index.dtype == torch.int64 else 32
 
 
 def embedding(table: torch.Tensor, index: torch.Tensor, scale: float = 1.0) -> torch.Tensor:

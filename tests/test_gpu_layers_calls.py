@@ -170,3 +170,16 @@ def test_a_bias_gradient_alone_leaves_out_the_weights(act, dtype):
     bl = b.clone().requires_grad_(True)
     (gb,) = torch.autograd.grad(layers.linear(x, w / 40, bl, activation=act), bl, yb)
     assert torch.equal(gb, only[2])
+
+
+def test_tensors_whose_sign_is_a_flag():
+    """The imaginary part of a conjugate is a view of the numbers with the sign kept beside them."""
+    c = torch.randn(50, 12, dtype=torch.complex64, generator=gen(2), device="cuda").conj()
+    x, w = c.imag, torch.randn(7, 12, generator=gen(3), device="cuda")
+    assert x.is_neg()
+    one = c[:, :1].imag
+    assert torch.equal(ops.linear(x, w), ops.linear(x.resolve_neg().contiguous(), w))
+    assert torch.equal(ops.linear(one, w[:, :1].contiguous()), ops.linear(one.resolve_neg().contiguous(), w[:, :1].contiguous()))
+    index = torch.randint(0, 50, (90,), generator=gen(4), device="cuda")
+    assert torch.equal(ops.embedding(one, index), one.resolve_neg()[index])
+    assert torch.equal(ops.embedding_backward(one, index[:50], 50), ops.embedding_backward(one.resolve_neg().contiguous(), index[:50], 50))
