@@ -41,10 +41,11 @@ def _staged(collective, tensors, group) -> None:
     if dist.get_backend(group) != "gloo" or not any(t.is_cuda for t in tensors):
         collective(*tensors)
         return
-    host = [t.cpu() for t in tensors]
-    collective(*host)
-    for t, h in zip(tensors, host):
-        t.copy_(h)
+    with torch.no_grad():                                  # parameters, too, are written in place
+        host = [t.cpu() for t in tensors]
+        collective(*host)
+        for t, h in zip(tensors, host):
+            t.copy_(h)
 
 
 def all_reduce(t: torch.Tensor, op=dist.ReduceOp.SUM, group: Optional[dist.ProcessGroup] = None) -> None:
