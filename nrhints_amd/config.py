@@ -142,7 +142,8 @@ def unsupported_reason(cfg: NeuSModelConfig) -> Optional[str]:
         # refuses that pair at call time)
         (not r.use_outside_nerf or (r.n_outside_samples == 32 and r.n_importance_samples == 64 and r.n_shadow_importance_clip == -1),
          "use_outside_nerf needs n_outside_samples = 32, the 128-sample layout and the hit-point shadow mode"),
-        # the default 8 x 256 / encodings 10 + 4 / skips [4] network runs on its compiled kernels, the others layer by layer (layers.linear)
+        # the default 8 x 256 / encodings 10 + 4 / skips [4] network runs on its compiled kernels, the others layer by layer (layers.linear);
+        # networks narrower than the compiled one stay refused, as they were before there was a layer chain to run them on
         (not r.use_outside_nerf or (n.d_hidden >= 256 and n.d_hidden % 2 == 0 and n.n_layers >= 2 and n.multi_res >= 1 and n.multi_res_view >= 1
                                     and all(0 <= i < n.n_layers - 1 for i in n.skips)),
          "outside_nerf: d_hidden even and at least 256, n_layers >= 2, multi_res and multi_res_view >= 1, skips among the layers before the last"),

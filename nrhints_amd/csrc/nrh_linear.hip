@@ -21,8 +21,8 @@
 //     is at most 2^-16 of the pair.  As float16 numbers, products of 2^-12 and 2^-13 would be zero and those past 65 504 infinite,
 //     though their sums fit the type (16 384 x 1 024 x 1 024: dx 108 us, dW 116 against 50 and 66 in float16).
 //     act' itself is kept in float32: no other rounding joins these, and a saturated unit's act' (1e-9 of a sigmoid at -20)
-//     keeps all its bits.  In parts, tiles are 128 x 256 (A, which is formed from two tensors, for as many columns as possible: 256 x 128 take 97 us
-//     where these take 77, 256 x 256 do not fit the registers).
+//     keeps all its bits.  In parts, large tiles are 128 x 256: A, which is formed from two tensors, for as many columns as fit (256 x 128
+//     take 97 us where these take 77; 256 x 256 spill registers, 98).
 //   * float32: x = x0 + x1 + x2 in three bfloat16 (each the rounded rest of the one before: 24 bits), and the six products x_a w_b
 //     with a + b <= 2 on v_mfma_f32_32x32x16_bf16.  What is left out is at most 2^-23 of |x w|, two of float32's own half steps
 //     (x1 w2 and x2 w1, 2^-24 each); six passes at the bf16 rate are 2.6 times the rate of v_mfma_f32_32x32x2_f32.  bfloat16 has
@@ -34,9 +34,9 @@
 // The MFMA's A role is played by the j operand, its rows permuted (column j = 16 h + 4 q + s of a block of 32 is MFMA row
 // 8 q + 4 h + s): a lane then holds 16 consecutive columns of ONE output row.
 // Measured: 16 384 x 1 024 x 1 024 bf16 38 us (0.9 PFLOP/s; a large library product reaches 1.6), 8 192 x 2 048 x 2 048 67 us (1.0);
-// 163 840 x 256 x 256 f32 147 us (146 TFLOP/s; the library's float32 products reach 154), of which writing the output is 42 and the six
-// bf16 products, at 1.3 PFLOP/s and 1.6 GHz under that load, the rest; 655 360 x 256 x 256 bf16 with a residual 218 us (1.0 GB at 4.6 TB/s, the
-// rate of a copy).  Small products are bound by the latency of their steps, about 0.4 us each.
+// 163 840 x 256 x 256 f32 145 us (148 TFLOP/s; the library's float32 products reach 154): of its 3.0e5 cycles (2.1 GHz) the MFMAs take 40 %
+// and vector instructions 36 %, mostly the three-way split, which every row tile repeats for W; 655 360 x 256 x 256 bf16 with a residual
+// 218 us (1.0 GB at 4.6 TB/s, the rate of a copy).  Small products are bound by the latency of their steps, about 0.4 us each.
 // A small output with a long reduction (every weight gradient) is split over the reduction; float32 partial tiles are joined in a
 // fixed order by reduce_kernel, so results do not depend on the order of execution.
 #include <hip/hip_runtime.h>
@@ -191,15 +191,17 @@ __device__ __forceinline__ float exp_minus(float a) {
   return __builtin_amdgcn_exp2f(-h) * fmaf(l, -0.693147182f, 1.0f);
 }
 
-// log(1 + e), 0 <= e <= 1: a series below 1/64 (the next term is under 2^-26 of it), above it log(u) e / (u - 1) of the rounded u = 1 + e
+// log(1 + e), 0 <= e <= 1: a series below 1/64 (the next term is under 2^-26 of it), above it log(u) e / (u - 1) of the rounded
+// u = 1 + e (Goldberg, What Every Computer Scientist Should Know About Floating-Point Arithmetic, theorem 4)
 __device__ __forceinline__ float log1p_unit(float e) {
   if (e < 0.015625f) return e * (1.0f - e * (0.5f - e * (0.333333343f - e * 0.25f)));
   const float u = 1.0f + e;
   return 0.693147182f * __builtin_amdgcn_logf(u) * (e * __builtin_amdgcn_rcpf(u - 1.0f));
 }
 
-// erfc(x), 0 <= x <= 14, as e^(-x^2) t P(t), t = 1 / (1 + x / 2): P is the polynomial of degree 8 with the least relative error over
-// that range (4.5e-8, by reweighted least squares on Chebyshev nodes in float64; 5.6 2^-24 as evaluated here).  ex2: e^(-x^2).
+// erfc(x), 0 <= x <= 14, as e^(-x^2) t P(t), t = 1 / (1 + x / 2) (the substitution of Press et al., Numerical Recipes, section 6.2): P
+// is the polynomial of degree 8 with the least relative error over that range (4.5e-8, by reweighted least squares on Chebyshev nodes in
+// float64; 5.6 2^-24 as evaluated here).  ex2: e^(-x^2).
 __device__ __forceinline__ float erfc_positive(float x, float ex2) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.0f));
   float q = fmaf(t, -0.05938727781f, 0.28612756729f);
