@@ -653,7 +653,8 @@ int nrh_sdf32_tables(const float* const* sdf_bias, const int* rows, const float*
  * nrh_linear_backward_data     xbar [m,k] = (ybar dact) w
  * nrh_linear_backward_weight   wbar [n,k] = (ybar dact)^T x, bias_bar [n] = column sums of ybar dact (may be null); m = 0 gives zeros.
  *   dact: null exactly for activation 0.  For ReLU it is used as a mask: anything positive exactly where z is (y itself, if there was
- *   no residual and y is not float16, where z up to 2^-25 rounds to zero).  ybar dact of 16-bit tensors is exact for none and ReLU, else 16 bits with float32's range.
+ *   no residual and y is not float16, where z up to 2^-25 rounds to zero).  ybar dact of 16-bit tensors is exact for none and ReLU, else
+ *   taken with 16 bits and float32's range; bias_bar sums it unrounded.
  *   Sums over rows are split in a way that depends on the sizes alone and joined in order: the same bits on every run.
  * workspace: nrh_linear_workspace_bytes(op = 0 forward, 1 backward_data, 2 backward_weight; ...) bytes, 16-byte aligned; -1: bad
  *   arguments; 0: none needed.  A workspace belongs to one call at a time.

@@ -183,3 +183,12 @@ def test_tensors_whose_sign_is_a_flag():
     index = torch.randint(0, 50, (90,), generator=gen(4), device="cuda")
     assert torch.equal(ops.embedding(one, index), one.resolve_neg()[index])
     assert torch.equal(ops.embedding_backward(one, index[:50], 50), ops.embedding_backward(one.resolve_neg().contiguous(), index[:50], 50))
+
+
+def test_a_bias_gradient_alone_of_no_rows_and_of_one():
+    """An empty batch gives zeros, one row gives itself, also from a column block of a wider buffer."""
+    wide, w = torch.randn(5, 20, generator=gen(1), device="cuda"), torch.randn(30, 8, generator=gen(2), device="cuda")
+    x, yb = wide[:, 3:11], torch.randn(5, 30, generator=gen(3), device="cuda")
+    for rows in (0, 1):
+        _, _, bb = ops.linear_backward(yb[:rows], x[:rows], w, None, want_x=False, want_weight=False)
+        assert torch.equal(bb, yb[:rows].sum(0))
